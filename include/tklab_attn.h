@@ -223,6 +223,97 @@ TK_API int tk_gqa_decode(const void* q, const void* k, const void* v, const int3
  * measurements and tests; returns TK_ERR_INVALID_ARGUMENT otherwise. */
 TK_API int tk_gqa_decode_set_path(int mode);
 
+/* Rotary positions on queries and keys (16-bit, head_dim a multiple of 8 up
+ * to 256) in one launch: pair i of a row, columns (i, i + r/2) or, when
+ * `interleaved`, (2i, 2i + 1), is rotated by the angle whose cosine and sine
+ * are row p of the fp32 tables (table_rows, r/2), r = rotary_dim (even, 2 to
+ * head_dim); columns from r on are copied.  p is positions[b, s] (int32, or
+ * int64 with positions_64), or s when positions is NULL; a p outside the
+ * tables leaves the row as it is and records TK_ERR_INVALID_ARGUMENT in the
+ * device status word.  `transpose` applies the transposed rotation (the
+ * input gradient).  q and k are strided (strides in elements over batch,
+ * head and row, multiples of 8; columns contiguous); q_out and k_out are
+ * contiguous (batch, heads, seq, head_dim) and may not overlap the inputs.
+ * k and k_out may be NULL with kv_heads 0. */
+TK_API int tk_rotary(const void* q, const void* k, void* q_out, void* k_out, const float* cos, const float* sin,
+                     const void* positions, int positions_64, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                     int64_t seq, int64_t head_dim, int64_t rotary_dim, int64_t table_rows,
+                     const int64_t* q_strides, const int64_t* k_strides, int dtype, int interleaved, int transpose,
+                     void* stream);
+
+/* Attention of a tree of drafted tokens (1 to 256 nodes) over a key/value
+ * cache, grouped query heads as in tk_gqa_decode (any q_heads = G * kv_heads):
+ *   q, o            (batch, q_heads, nodes, head_dim) contiguous
+ *   k, v            (batch, kv_heads, seq_kv, head_dim) cache
+ *   k_tree, v_tree  (batch, kv_heads, nodes, head_dim) the tree's own rows
+ *   strides         12 element strides: k, v, k_tree, v_tree x (batch, head,
+ *                   row), multiples of 8; columns contiguous
+ *   kv_lens         (batch) int32 valid cache rows, clamped to [0, seq_kv]
+ *   parents         (batch, nodes) int32 with a stride of parent_stride
+ *                   (nodes, or 0 for one tree shared by all), parents[t] < t,
+ *                   anything else a root; NULL: a chain (parents[t] = t - 1)
+ *   tree_sizes      (batch) int32 nodes in use, or NULL; the rest get o = 0,
+ *                   lse = -inf
+ *   lse             (batch, q_heads, nodes) fp32 base-2 log-sum-exp, or NULL
+ * Node t attends the valid cache rows, its ancestors and itself.  Cache rows
+ * past kv_lens and tree rows past tree_sizes may hold anything, NaN included.
+ * head_dim a multiple of 8 up to 128.  `workspace`: at least
+ * tk_tree_attn_workspace_bytes(...) bytes, 256-byte aligned, private to this
+ * call until it completes (NULL when that is 0). */
+TK_API size_t tk_tree_attn_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes,
+                                           int64_t seq_kv, int64_t head_dim);
+TK_API int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree, const void* v_tree,
+                        const int64_t* strides, const int32_t* kv_lens, const int32_t* parents,
+                        int64_t parent_stride, const int32_t* tree_sizes, void* o, float* lse, void* workspace,
+                        size_t workspace_bytes, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes,
+                        int64_t seq_kv, int64_t head_dim, int dtype, float scale, void* stream);
+
+/* Element type of probabilities (tk_verify_draft). */
+#define TK_PROB_F16 0
+#define TK_PROB_BF16 1
+#define TK_PROB_F32 2
+
+/* Verification of drafted tokens (1 to 256 nodes) against the target's
+ * probabilities.
+ * Node 0 is the last known token; node c > 0 carries tokens[b, c], drafted
+ * after its parent (parents as in tk_tree_attn).  target (batch, nodes,
+ * vocab): row n the target's distribution after node n.  draft (batch,
+ * nodes - 1, vocab) or NULL: row n the distribution that node n + 1 was drawn
+ * from; chains (parents NULL) only.  target_strides and draft_strides:
+ * element strides over batch and node; the vocabulary is contiguous.
+ * From node 0 on, children are tried in index order: accepted if
+ * u (1 - S) < p(x) with u = uniforms[b, c], S the mass under p of the
+ * different tokens of its earlier siblings (a token already tried is
+ * refused), or with draft if u q(x) < p(x).  The next token is
+ * argmax_v w_v / noise[b, v] (lowest index of equals; noise: positive
+ * exponential variates, (batch, vocab) fp32) with w = p without the tried
+ * tokens, max(p - q, 0) with draft, p at a node without children and where w
+ * has no positive entry.  Tokens outside the vocabulary are refused; NaN
+ * counts as no probability.
+ *   path       (batch, nodes) int32: accepted nodes from node 0 on, then -1
+ *   path_lens  (batch) int32: how many (node 0 counts)
+ *   next       (batch) next token, the type of tokens (int64 with tokens_64);
+ *              -1 for a sequence with tree_sizes[b] = 0 */
+TK_API int tk_verify_draft(const void* target, const int64_t* target_strides, const void* draft,
+                           const int64_t* draft_strides, const void* tokens, int tokens_64, const int32_t* parents,
+                           int64_t parent_stride, const int32_t* tree_sizes, const float* uniforms,
+                           const float* noise, int32_t* path, int32_t* path_lens, void* next, int64_t batch,
+                           int64_t nodes, int64_t vocab, int prob_type, void* stream);
+
+/* Accepted rows into the cache, in one launch for all layers: row path[b, i]
+ * (i < path_lens[b]) of k_tree and v_tree (layers, batch, kv_heads, nodes,
+ * head_dim) goes to row kv_lens[b] + i of k and v (layers, batch, kv_heads,
+ * seq_kv, head_dim), and new_lens[b] = kv_lens[b] + path_lens[b].  strides: 16
+ * element strides, k, v, k_tree, v_tree x (layer, batch, head, row), multiples
+ * of 8.  Rows that the cache has no room for are not written, new_lens stops
+ * at seq_kv and TK_ERR_TOO_LARGE goes to the device status word; a path entry
+ * outside [0, nodes) is skipped with TK_ERR_INVALID_ARGUMENT.  new_lens may
+ * not be kv_lens. */
+TK_API int tk_commit_draft(void* k, void* v, const void* k_tree, const void* v_tree, const int64_t* strides,
+                           const int32_t* path, const int32_t* path_lens, const int32_t* kv_lens, int32_t* new_lens,
+                           int64_t layers, int64_t batch, int64_t kv_heads, int64_t nodes, int64_t seq_kv,
+                           int64_t head_dim, void* stream);
+
 /* Bytes of the fp32 dQ accumulator tk_attn_bwd needs (0 on bad sizes). */
 TK_API size_t tk_attn_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t seq, int64_t head_dim);
 

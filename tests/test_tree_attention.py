@@ -1,0 +1,279 @@
+"""``tklab.kernels.tree_attention`` against the 64-bit reference (GPU), and its refusals (CPU)."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from oracle.speculative_oracle import tree_attention_reference
+from tklab import _native
+from tklab.kernels.flash_attention import check_device_status
+from tklab.kernels.gqa_decode import gqa_decode
+from tklab.kernels.tree_attention import tree_attention
+
+gpu = pytest.mark.skipif(not torch.cuda.is_available(), reason="CUDA GPU is required")
+ROUND = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+
+
+def problem(batch, q_heads, kv_heads, nodes, dim, capacity, lens, dtype, *, seed=0, tree=True, spread=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    rand = lambda *shape: torch.randn(*shape, generator=gen).to(dtype)  # noqa: E731
+    parents = None
+    if tree:
+        index = torch.arange(nodes)
+        parents = torch.minimum((torch.rand(batch, nodes, generator=gen).sqrt() * index).floor(), (index - 1).clamp_min(0)).int()
+        parents[:, 0] = -1
+    return {
+        "q": (spread * rand(batch, q_heads, nodes, dim)).to(dtype),
+        "k_cache": rand(batch, kv_heads, capacity, dim), "v_cache": rand(batch, kv_heads, capacity, dim),
+        "k_tree": rand(batch, kv_heads, nodes, dim), "v_tree": rand(batch, kv_heads, nodes, dim),
+        "kv_lens": torch.tensor(lens, dtype=torch.int32), "parents": parents,
+    }
+
+
+def on_gpu(p):
+    return {n: None if t is None else t.cuda() for n, t in p.items()}
+
+
+def assert_attends(o, lse, ref):
+    """P and o are rounded to the 16-bit type once each; the fp32 arithmetic (scores, exponentials, sums) stays below
+    2^-12 of the weighted magnitude at these sizes; 16-bit P below 2^-14 (float16) adds 2^-25 a key at most."""
+    ref_o, ref_lse, spread = ref
+    bound = (2.0 * ROUND[o.dtype] + 2.0**-12) * spread + 2.0**-14 * 2.0**-3
+    err = (o.double().cpu() - ref_o).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+    if lse is not None:
+        empty = torch.isinf(ref_lse)
+        assert torch.equal(torch.isinf(lse.cpu()), empty) and bool((lse.cpu()[empty] < 0).all())
+        off = (lse.double().cpu() - ref_lse)[~empty].abs()
+        assert not off.numel() or float((off - 1e-6 * ref_lse[~empty].abs()).max()) <= 2e-4
+
+
+def check(p, **kwargs):
+    o, lse = tree_attention(**on_gpu(p), return_lse=True, **{n: v.cuda() if torch.is_tensor(v) else v for n, v in kwargs.items()})
+    assert o.shape == p["q"].shape and o.dtype == p["q"].dtype
+    assert_attends(o, lse, tree_attention_reference(**p, **kwargs))
+    check_device_status()
+    return o, lse
+
+
+# ---------------------------------------------------------------- refusals
+def test_refuses_bad_arguments() -> None:
+    p = problem(2, 4, 2, 3, 64, 16, [4, 5], torch.float16)
+
+    def bad(match, **change):
+        with pytest.raises(ValueError, match=match):
+            tree_attention(**{**p, **change})
+
+    bad("4-dimensional", q=p["q"][0])
+    bad("identical", v_cache=p["v_cache"][:, :1])
+    bad("the tree's", k_tree=p["k_tree"][:, :, :2])
+    bad("empty", q=p["q"][:, :, :0], k_tree=p["k_tree"][:, :, :0], v_tree=p["v_tree"][:, :, :0])
+    bad("multiple of kv_heads", q=p["q"][:, :3])
+    bad("share one dtype", q=p["q"].float())
+    bad("share one dtype", v_tree=p["v_tree"].bfloat16())
+    bad("CUDA")
+    big = problem(1, 1, 1, 257, 8, 8, [1], torch.float16)
+    with pytest.raises(ValueError, match="256 nodes"):
+        tree_attention(**big)
+    wide = problem(1, 1, 1, 2, 136, 8, [1], torch.float16)
+    with pytest.raises(ValueError, match="head_dim"):
+        tree_attention(**wide)
+
+
+@pytest.mark.parametrize(
+    ("kwargs", "status"),
+    [
+        ({"q": None}, 1), ({"kv_lens": None}, 1), ({"strides": None}, 1), ({"batch": 0}, 1), ({"q_heads": 3}, 1),
+        ({"nodes": 0}, 1), ({"scale": 0.0}, 1), ({"scale": float("nan")}, 1), ({"parent_stride": 2}, 1),
+        ({"head_dim": 20}, 2), ({"head_dim": 136}, 2), ({"nodes": 257, "parent_stride": 257}, 2), ({"dtype": 3}, 2),
+        ({"o": 0x1008}, 3), ({"lse": 0x1002}, 3), ({"kv_lens": 0x1001}, 3), ({"workspace": 0x1010}, 3),
+        ({"seq_kv": 1 << 31}, 8),
+    ],
+)
+def test_library_refuses_before_launch(kwargs: dict, status: int) -> None:
+    args = {"q": 0x1000, "k": 0x1000, "v": 0x1000, "k_tree": 0x1000, "v_tree": 0x1000,
+            "strides": (ctypes.c_int64 * 12)(*[64] * 12), "kv_lens": 0x1000, "parents": 0x1000, "parent_stride": 3,
+            "tree_sizes": None, "o": 0x1000, "lse": None, "workspace": None, "workspace_bytes": 0, "batch": 1,
+            "q_heads": 4, "kv_heads": 2, "nodes": 3, "seq_kv": 16, "head_dim": 64, "dtype": 1, "scale": 0.125,
+            "stream": None}
+    args.update(kwargs)
+    assert _native.load().tk_tree_attn(*args.values()) == status
+
+
+# --------------------------------------------------------------------- GPU
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group", [1, 3, 4, 8])
+@pytest.mark.parametrize("nodes", [1, 2, 7, 16, 33, 64])
+def test_matches_reference(dtype: torch.dtype, dim: int, group: int, nodes: int) -> None:
+    lens = [0, 1, 127, 128, 129, 300]
+    check(problem(6, 2 * group, 2, nodes, dim, 301, lens, dtype, seed=nodes + group))
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("dim", [8, 24, 40, 72, 96, 120])
+def test_odd_head_dims(dim: int) -> None:
+    check(problem(2, 6, 2, 11, dim, 200, [150, 64], torch.bfloat16, seed=dim))
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize(("group", "nodes"), [(1, 127), (1, 128), (1, 129), (2, 200), (3, 256), (16, 33), (16, 40), (5, 77)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_many_rows(group: int, nodes: int, tree: bool) -> None:
+    """More rows than one tile of 128, trees of more than one tile, chains and trees."""
+    check(problem(2, group, 1, nodes, 64, 400, [400, 77], torch.float16, seed=nodes, tree=tree))
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize(("batch", "capacity", "nodes"), [(1, 5000, 5), (3, 3333, 20), (1, 20000, 1)])
+def test_split_lengths(dim: int, batch: int, capacity: int, nodes: int) -> None:
+    """Long caches, split over many CTAs; scores that grow along the cache move the running maxima."""
+    lens = [capacity, capacity // 3, 1][:batch]
+    p = problem(batch, 8, 2, nodes, dim, capacity, lens, torch.bfloat16, seed=capacity)
+    p["k_cache"] = (p["k_cache"].float() * torch.linspace(0.1, 2.5, capacity)[None, None, :, None]).bfloat16()
+    o, lse = check(p)
+    o2, lse2 = tree_attention(**on_gpu(p), return_lse=True)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)  # the same bits every time
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("batch", [40, 200])
+def test_many_sequences_of_mixed_length(batch: int) -> None:
+    lens = [(37 * i * i + 11) % 601 for i in range(batch)]
+    check(problem(batch, 4, 2, 6, 64, 600, lens, torch.bfloat16, seed=batch))  # one length above the capacity's use, some 0
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_unused_rows_may_hold_anything(bad: float, dim: int) -> None:
+    p = problem(4, 8, 2, 9, dim, 300, [300, 150, 0, 129], torch.bfloat16, seed=3)
+    sizes = torch.tensor([9, 4, 1, 0], dtype=torch.int32)
+    clean = check(p, tree_sizes=sizes)
+    for b in range(4):
+        for name in ("k", "v"):
+            p[name + "_cache"][b, :, int(p["kv_lens"][b]) :] = bad
+            p[name + "_tree"][b, :, int(sizes[b]) :] = bad
+        p["q"][b, :, int(sizes[b]) :] = bad
+    dirty = tree_attention(**on_gpu(p), tree_sizes=sizes.cuda(), return_lse=True)
+    for a, b in zip(clean, dirty, strict=True):
+        assert torch.equal(a, b)
+    assert bool((dirty[0][3] == 0).all()) and bool((dirty[0][1, :, 4:] == 0).all())
+    check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+def test_lengths_past_the_cache_and_below_zero_are_clamped() -> None:
+    p = problem(2, 4, 2, 3, 64, 100, [100, 0], torch.float16, seed=8)
+    o = tree_attention(**on_gpu(p))
+    p["kv_lens"] = torch.tensor([1000, -5], dtype=torch.int32)
+    assert torch.equal(o, tree_attention(**on_gpu(p)))
+    full = torch.tensor([99, -1], dtype=torch.int32)
+    o = tree_attention(**on_gpu(p), tree_sizes=full.cuda())
+    assert torch.equal(o, tree_attention(**on_gpu(p), tree_sizes=full.clamp(0, 3).cuda()))
+    check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+def test_parents_forms() -> None:
+    """A chain given as parents, one tree for the batch, several roots, parents that are none."""
+    p = problem(3, 4, 2, 12, 64, 90, [90, 10, 33], torch.bfloat16, seed=4, tree=False)
+    o = tree_attention(**on_gpu(p))
+    chain = torch.arange(-1, 11, dtype=torch.int32)
+    assert torch.equal(o, tree_attention(**on_gpu({**p, "parents": chain})))
+    assert torch.equal(o, tree_attention(**on_gpu({**p, "parents": chain.expand(3, 12)})))
+    odd = torch.tensor([-1, -1, 0, 1, 9, 5, 2, -7, 3, 3, 2**30, 10], dtype=torch.int32)
+    check({**p, "parents": odd})
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_strided_caches_and_trees(dtype: torch.dtype) -> None:
+    p = problem(3, 8, 4, 5, 64, 70, [70, 1, 40], dtype, seed=12)
+    ref = tree_attention(**on_gpu(p))
+    g = on_gpu(p)
+    # (batch, rows, heads, dim) storage seen as (batch, heads, rows, dim); K and V interleaved; padded rows.
+    bshd = {n: g[n].transpose(1, 2).contiguous().transpose(1, 2) for n in ("k_cache", "v_cache", "k_tree", "v_tree")}
+    assert torch.equal(ref, tree_attention(**{**g, **bshd}))
+    both = torch.stack((g["k_cache"], g["v_cache"]), 2)
+    assert torch.equal(ref, tree_attention(**{**g, "k_cache": both[:, :, 0], "v_cache": both[:, :, 1]}))
+    padded = torch.nn.functional.pad(g["v_cache"], (8, 16))[..., 8:72]
+    assert torch.equal(ref, tree_attention(**{**g, "v_cache": padded}))
+    odd = torch.nn.functional.pad(g["k_tree"], (1, 2))[..., 1:65]
+    assert torch.equal(ref, tree_attention(**{**g, "k_tree": odd, "q": torch.nn.functional.pad(g["q"], (3, 0))[..., 3:]}))
+    with pytest.raises(ValueError, match="the K cache"):
+        tree_attention(**{**g, "k_cache": torch.nn.functional.pad(g["k_cache"], (1, 2))[..., 1:65]})
+    with pytest.raises(ValueError, match="the V cache"):
+        tree_attention(**{**g, "v_cache": g["v_cache"][:, :1].expand(3, 4, 70, 64)})
+    check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+def test_one_node_equals_decode_of_the_extended_cache() -> None:
+    p = on_gpu(problem(2, 16, 4, 1, 128, 500, [400, 77], torch.bfloat16, seed=2))
+    o, lse = tree_attention(**p, return_lse=True)
+    for b, n in enumerate((400, 77)):
+        p["k_cache"][b, :, n], p["v_cache"][b, :, n] = p["k_tree"][b, :, 0], p["v_tree"][b, :, 0]
+    o2, lse2 = gqa_decode(p["q"], p["k_cache"], p["v_cache"], kv_lens=p["kv_lens"] + 1, return_lse=True)
+    assert (o.float() - o2.float()).abs().max().item() <= 1e-2
+    assert torch.allclose(lse[:, :, 0], lse2, atol=1e-3)
+    check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+def test_scale_large_scores_and_other_streams() -> None:
+    p = problem(2, 4, 2, 6, 64, 333, [333, 200], torch.float16, seed=15, spread=6.0)
+    check(p, scale=0.3)
+    g = on_gpu(p)
+    ref = tree_attention(**g, scale=0.3)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        o = tree_attention(**g, scale=0.3)
+    side.synchronize()
+    assert torch.equal(o, ref)
+
+
+@pytest.mark.gpu
+@gpu
+def test_rows_past_32_bit_offsets() -> None:
+    """The last rows of a cache of more than 2^31 elements."""
+    capacity, dim = 2**31 // 128 // 2 + 1000, 128
+    cache = torch.zeros(1, 2, capacity, dim, dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    last = torch.randn(500, dim, generator=gen, device="cuda").bfloat16()
+    cache[0, 1, -500:] = last
+    view = cache[:, 1:, :]  # starts past 2^30 elements
+    whole = torch.cat((cache[:, 1:, :1], cache[:, 1:, -500:]), 2)
+    q = torch.randn(1, 2, 3, dim, generator=gen, device="cuda").bfloat16()
+    tree = torch.randn(1, 1, 3, dim, generator=gen, device="cuda").bfloat16()
+    lens = torch.tensor([capacity], dtype=torch.int32, device="cuda")
+    # Zero keys score 0 and carry zero values: they only add their count to the sum.
+    o, lse = tree_attention(q, view, view, tree, tree, lens, return_lse=True)
+    zeros = capacity - 501
+    ref_o, ref_lse, _ = tree_attention_reference(q.cpu(), whole.cpu(), whole.cpu(), tree.cpu(), tree.cpu(), torch.tensor([501]))
+    total = torch.exp2(ref_lse) + zeros
+    assert torch.allclose(lse.double().cpu(), torch.log2(total), atol=1e-3)
+    expect = ref_o * (torch.exp2(ref_lse) / total)[..., None]
+    assert (o.double().cpu() - expect).abs().max().item() <= 2.0**-7 * float(expect.abs().max()) + 1e-6
+    both = tree_attention(q.repeat(1, 2, 1, 1), cache, cache, tree.repeat(1, 2, 1, 1), tree.repeat(1, 2, 1, 1), lens)
+    assert torch.equal(both[:, 2:], o)
+    check_device_status()

@@ -387,6 +387,196 @@ int tk_gqa_decode_set_path(int mode) {
   return tk::kOk;
 }
 
+int tk_rotary(const void* q, const void* k, void* q_out, void* k_out, const float* cos, const float* sin,
+              const void* positions, int positions_64, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq,
+              int64_t head_dim, int64_t rotary_dim, int64_t table_rows, const int64_t* q_strides,
+              const int64_t* k_strides, int dtype, int interleaved, int transpose, void* stream) {
+  if (q == nullptr || q_out == nullptr || cos == nullptr || sin == nullptr || q_strides == nullptr)
+    return tk::kErrInvalidArgument;
+  if (kv_heads < 0 || (kv_heads > 0 && (k == nullptr || k_out == nullptr || k_strides == nullptr)))
+    return tk::kErrInvalidArgument;
+  if (int rc = check_shape(batch, q_heads + kv_heads, seq, head_dim, dtype, 256)) return rc;
+  if (q_heads <= 0 || table_rows <= 0) return tk::kErrInvalidArgument;
+  if (rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2 != 0) return tk::kErrUnsupported;
+  if (positions == nullptr && table_rows < seq) return tk::kErrInvalidArgument;
+  if (table_rows > INT_MAX) return tk::kErrTooLarge;
+  if (!aligned16(q) || !aligned16(q_out) || !aligned16(cos) || !aligned16(sin)) return tk::kErrMisaligned;
+  if (kv_heads > 0 && (!aligned16(k) || !aligned16(k_out))) return tk::kErrMisaligned;
+  if (reinterpret_cast<uintptr_t>(positions) & (positions_64 ? 7u : 3u)) return tk::kErrMisaligned;
+  tk::RotaryArgs a{};
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = q_strides[i];
+    a.k_stride[i] = kv_heads > 0 ? k_strides[i] : 0;
+    if (a.q_stride[i] % 8 != 0 || a.k_stride[i] % 8 != 0) return tk::kErrMisaligned;
+  }
+  if (int rc = status_ptr(&a.status)) return rc;
+  a.q = q;
+  a.k = k;
+  a.q_out = q_out;
+  a.k_out = k_out;
+  a.cos = cos;
+  a.sin = sin;
+  a.positions = positions;
+  a.B = batch;
+  a.Hq = q_heads;
+  a.Hkv = kv_heads;
+  a.S = seq;
+  a.D = head_dim;
+  a.rotary_dim = rotary_dim;
+  a.table_rows = table_rows;
+  a.bf16 = dtype == TK_DTYPE_BF16;
+  a.interleaved = interleaved != 0;
+  a.transpose = transpose != 0;
+  a.positions_64 = positions_64 != 0;
+  a.stream = static_cast<cudaStream_t>(stream);
+  return tk::launch_rotary(a);
+}
+
+size_t tk_tree_attn_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes, int64_t seq_kv,
+                                    int64_t head_dim) {
+  (void)batch, (void)q_heads, (void)kv_heads, (void)nodes, (void)seq_kv, (void)head_dim;
+  return 0;
+}
+
+int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree, const void* v_tree,
+                 const int64_t* strides, const int32_t* kv_lens, const int32_t* parents, int64_t parent_stride,
+                 const int32_t* tree_sizes, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                 int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes, int64_t seq_kv, int64_t head_dim,
+                 int dtype, float scale, void* stream) {
+  if (q == nullptr || k == nullptr || v == nullptr || k_tree == nullptr || v_tree == nullptr || strides == nullptr ||
+      kv_lens == nullptr || o == nullptr)
+    return tk::kErrInvalidArgument;
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || nodes <= 0 || seq_kv <= 0 || q_heads % kv_heads != 0)
+    return tk::kErrInvalidArgument;
+  if (parents != nullptr && parent_stride != 0 && parent_stride < nodes) return tk::kErrInvalidArgument;
+  if (head_dim < 8 || head_dim > 128 || head_dim % 8 != 0 || nodes > tk::kTreeMaxNodes) return tk::kErrUnsupported;
+  if (dtype != TK_DTYPE_F16 && dtype != TK_DTYPE_BF16) return tk::kErrUnsupported;
+  if (!std::isfinite(scale) || scale <= 0.0f) return tk::kErrInvalidArgument;
+  if (seq_kv > (1 << 30) || batch > (1 << 20) || q_heads > (1 << 20) || batch * q_heads * nodes > (1 << 30))
+    return tk::kErrTooLarge;
+  for (const void* p : {q, k, v, k_tree, v_tree, static_cast<const void*>(o)})
+    if (!aligned16(p)) return tk::kErrMisaligned;
+  for (const void* p : {static_cast<const void*>(kv_lens), static_cast<const void*>(parents),
+                        static_cast<const void*>(tree_sizes), static_cast<const void*>(lse)})
+    if (reinterpret_cast<uintptr_t>(p) & 3u) return tk::kErrMisaligned;
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return tk::kErrMisaligned;
+  if (workspace_bytes < tk_tree_attn_workspace_bytes(batch, q_heads, kv_heads, nodes, seq_kv, head_dim))
+    return tk::kErrInvalidArgument;
+  tk::TreeAttnArgs a{};
+  for (int i = 0; i < 12; ++i) {
+    if (strides[i] < 0 || strides[i] % 8 != 0) return tk::kErrMisaligned;
+    a.strides[i] = strides[i];
+  }
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.k_tree = k_tree;
+  a.v_tree = v_tree;
+  a.kv_lens = kv_lens;
+  a.parents = parents;
+  a.tree_sizes = tree_sizes;
+  a.o = o;
+  a.lse = lse;
+  a.parent_stride = parent_stride;
+  a.B = batch;
+  a.Hkv = kv_heads;
+  a.G = q_heads / kv_heads;
+  a.T = nodes;
+  a.L = seq_kv;
+  a.D = head_dim;
+  a.bf16 = dtype == TK_DTYPE_BF16;
+  a.scale_log2 = scale * kLog2e;
+  a.stream = static_cast<cudaStream_t>(stream);
+  return tk::launch_tree_attn(a);
+}
+
+int tk_verify_draft(const void* target, const int64_t* target_strides, const void* draft,
+                    const int64_t* draft_strides, const void* tokens, int tokens_64, const int32_t* parents,
+                    int64_t parent_stride, const int32_t* tree_sizes, const float* uniforms, const float* noise,
+                    int32_t* path, int32_t* path_lens, void* next, int64_t batch, int64_t nodes, int64_t vocab,
+                    int prob_type, void* stream) {
+  if (target == nullptr || target_strides == nullptr || tokens == nullptr || uniforms == nullptr ||
+      noise == nullptr || path == nullptr || path_lens == nullptr || next == nullptr)
+    return tk::kErrInvalidArgument;
+  if (draft != nullptr && (draft_strides == nullptr || parents != nullptr)) return tk::kErrInvalidArgument;
+  if (batch <= 0 || nodes <= 0 || vocab <= 0) return tk::kErrInvalidArgument;
+  if (parents != nullptr && parent_stride != 0 && parent_stride < nodes) return tk::kErrInvalidArgument;
+  if (prob_type != TK_PROB_F16 && prob_type != TK_PROB_BF16 && prob_type != TK_PROB_F32) return tk::kErrUnsupported;
+  if (nodes > tk::kTreeMaxNodes) return tk::kErrUnsupported;
+  if (batch > (1 << 20) || vocab > (1 << 30)) return tk::kErrTooLarge;
+  const uintptr_t prob_mask = prob_type == TK_PROB_F32 ? 3u : 1u, token_mask = tokens_64 ? 7u : 3u;
+  if ((reinterpret_cast<uintptr_t>(target) & prob_mask) || (reinterpret_cast<uintptr_t>(draft) & prob_mask) ||
+      (reinterpret_cast<uintptr_t>(tokens) & token_mask) || (reinterpret_cast<uintptr_t>(next) & token_mask))
+    return tk::kErrMisaligned;
+  for (const void* p : {static_cast<const void*>(parents), static_cast<const void*>(tree_sizes),
+                        static_cast<const void*>(uniforms), static_cast<const void*>(noise),
+                        static_cast<const void*>(path), static_cast<const void*>(path_lens)})
+    if (reinterpret_cast<uintptr_t>(p) & 3u) return tk::kErrMisaligned;
+  tk::VerifyArgs a{};
+  a.target = target;
+  a.draft = nodes > 1 ? draft : nullptr;
+  a.tokens = tokens;
+  a.parents = parents;
+  a.tree_sizes = tree_sizes;
+  a.uniforms = uniforms;
+  a.noise = noise;
+  a.path = path;
+  a.path_lens = path_lens;
+  a.next = next;
+  for (int i = 0; i < 2; ++i) {
+    a.target_stride[i] = target_strides[i];
+    a.draft_stride[i] = draft != nullptr ? draft_strides[i] : 0;
+  }
+  a.parent_stride = parent_stride;
+  a.B = batch;
+  a.T = nodes;
+  a.V = vocab;
+  a.type = prob_type;
+  a.tokens_64 = tokens_64 != 0;
+  a.stream = static_cast<cudaStream_t>(stream);
+  return tk::launch_verify(a);
+}
+
+int tk_commit_draft(void* k, void* v, const void* k_tree, const void* v_tree, const int64_t* strides,
+                    const int32_t* path, const int32_t* path_lens, const int32_t* kv_lens, int32_t* new_lens,
+                    int64_t layers, int64_t batch, int64_t kv_heads, int64_t nodes, int64_t seq_kv, int64_t head_dim,
+                    void* stream) {
+  if (k == nullptr || v == nullptr || k_tree == nullptr || v_tree == nullptr || strides == nullptr ||
+      path == nullptr || path_lens == nullptr || kv_lens == nullptr || new_lens == nullptr || new_lens == kv_lens)
+    return tk::kErrInvalidArgument;
+  if (layers <= 0 || batch <= 0 || kv_heads <= 0 || nodes <= 0 || seq_kv <= 0 || head_dim <= 0)
+    return tk::kErrInvalidArgument;
+  if (head_dim % 8 != 0 || head_dim > 256 || nodes > tk::kTreeMaxNodes) return tk::kErrUnsupported;
+  if (layers > (1 << 15) || batch > (1 << 15) || kv_heads > 65535 || seq_kv > (1 << 30)) return tk::kErrTooLarge;
+  for (const void* p : {static_cast<const void*>(k), static_cast<const void*>(v), k_tree, v_tree})
+    if (!aligned16(p)) return tk::kErrMisaligned;
+  for (const void* p : {static_cast<const void*>(path), static_cast<const void*>(path_lens),
+                        static_cast<const void*>(kv_lens), static_cast<const void*>(new_lens)})
+    if (reinterpret_cast<uintptr_t>(p) & 3u) return tk::kErrMisaligned;
+  tk::CommitArgs a{};
+  for (int i = 0; i < 16; ++i) {
+    if (strides[i] < 0 || strides[i] % 8 != 0) return tk::kErrMisaligned;
+    a.strides[i] = strides[i];
+  }
+  if (int rc = status_ptr(&a.status)) return rc;
+  a.k = k;
+  a.v = v;
+  a.k_tree = k_tree;
+  a.v_tree = v_tree;
+  a.path = path;
+  a.path_lens = path_lens;
+  a.kv_lens = kv_lens;
+  a.new_lens = new_lens;
+  a.layers = layers;
+  a.B = batch;
+  a.H = kv_heads;
+  a.T = nodes;
+  a.L = seq_kv;
+  a.D = head_dim;
+  a.stream = static_cast<cudaStream_t>(stream);
+  return tk::launch_commit(a);
+}
+
 int tk_attn_dq_convert(const float* dq_accum, void* dq, int64_t n, int dtype, void* stream) {
   if (dq_accum == nullptr || dq == nullptr || n <= 0 || n % 8 != 0) return tk::kErrInvalidArgument;
   if (dtype != TK_DTYPE_F16 && dtype != TK_DTYPE_BF16) return tk::kErrUnsupported;

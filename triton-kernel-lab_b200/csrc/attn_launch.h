@@ -181,6 +181,85 @@ struct GqaDecodeArgs {
   const CUtensorMap* tm_v = nullptr;
 };
 
+// Rotary positions (rotary_sm100.cu).  Strides in elements: batch, head, row.
+struct RotaryArgs {
+  const void* q;
+  const void* k;  // nullptr with Hkv = 0: queries only
+  void* q_out;    // contiguous (B, Hq, S, D)
+  void* k_out;    // contiguous (B, Hkv, S, D)
+  const float* cos;
+  const float* sin;  // (table_rows, rotary_dim / 2)
+  const void* positions;  // (B, S) int32 or int64, or nullptr: 0..S-1
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t B, Hq, Hkv, S, D, rotary_dim, table_rows;
+  bool bf16, interleaved, transpose, positions_64;
+  int* status;
+  cudaStream_t stream;
+};
+
+// Nodes of a drafted tree at most (the attention keeps a bit per node and row).
+constexpr int kTreeMaxNodes = 256;
+
+// Tree attention over a cache (tree_attn_sm100.cu).
+struct TreeAttnArgs {
+  const void* q;       // (B, Hkv * G, T, D)
+  const void* k;       // cache (B, Hkv, L, D), strided
+  const void* v;
+  const void* k_tree;  // (B, Hkv, T, D), strided
+  const void* v_tree;
+  const int* kv_lens;     // (B)
+  const int* parents;     // (B or 1, T), or nullptr: a chain
+  const int* tree_sizes;  // (B), or nullptr: T each
+  void* o;                // (B, Hkv * G, T, D)
+  float* lse;             // (B, Hkv * G, T), or nullptr
+  int64_t parent_stride;  // T, or 0 for one tree shared by all sequences
+  int64_t strides[12];    // elements: k, v, k_tree, v_tree x (batch, head, row)
+  int64_t B, Hkv, G, T, L, D;
+  bool bf16;
+  float scale_log2;
+  cudaStream_t stream;
+};
+
+// Verification of drafted tokens and the cache commit (speculative_sm100.cu).
+constexpr int kProbF16 = 0, kProbBf16 = 1, kProbF32 = 2;
+struct VerifyArgs {
+  const void* target;  // (B, T, V), strided over batch and node
+  const void* draft;   // (B, T - 1, V), strided, or nullptr
+  const void* tokens;  // (B, T) int32 or int64
+  const int* parents;
+  const int* tree_sizes;
+  const float* uniforms;  // (B, T)
+  const float* noise;     // (B, V)
+  int* path;              // (B, T)
+  int* path_lens;         // (B)
+  void* next;             // (B), the tokens' type
+  int64_t target_stride[2], draft_stride[2], parent_stride;
+  int64_t B, T, V;
+  int type;
+  bool tokens_64;
+  cudaStream_t stream;
+};
+
+struct CommitArgs {
+  void* k;  // caches (layers, B, H, L, D), strided
+  void* v;
+  const void* k_tree;  // (layers, B, H, T, D), strided
+  const void* v_tree;
+  const int* path;       // (B, T)
+  const int* path_lens;  // (B)
+  const int* kv_lens;    // (B)
+  int* new_lens;         // (B)
+  int64_t strides[16];   // elements: k, v, k_tree, v_tree x (layer, batch, head, row)
+  int64_t layers, B, H, T, L, D;
+  int* status;
+  cudaStream_t stream;
+};
+
+int launch_rotary(const RotaryArgs& a);
+int launch_tree_attn(const TreeAttnArgs& a);
+int launch_verify(const VerifyArgs& a);
+int launch_commit(const CommitArgs& a);
 int launch_attn_fwd(const FwdArgs& a);
 // Bytes of workspace the forward's key-split schedule needs for this problem
 // on a device with `sms` SMs (0: the problem is not split).

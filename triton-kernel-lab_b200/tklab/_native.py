@@ -97,6 +97,32 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ],
     ),
     "tk_gqa_decode_set_path": (ctypes.c_int, [ctypes.c_int]),
+    "tk_rotary": (
+        ctypes.c_int,
+        [
+            _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+            ctypes.POINTER(_i64), ctypes.POINTER(_i64), ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp,
+        ],
+    ),
+    "tk_tree_attn_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "tk_tree_attn": (
+        ctypes.c_int,
+        [
+            _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(_i64), _vp, _vp, _i64, _vp, _vp, _vp, _vp, ctypes.c_size_t,
+            _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_float, _vp,
+        ],
+    ),
+    "tk_verify_draft": (
+        ctypes.c_int,
+        [
+            _vp, ctypes.POINTER(_i64), _vp, ctypes.POINTER(_i64), _vp, ctypes.c_int, _vp, _i64, _vp, _vp, _vp,
+            _vp, _vp, _vp, _i64, _i64, _i64, ctypes.c_int, _vp,
+        ],
+    ),
+    "tk_commit_draft": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, ctypes.POINTER(_i64), _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp],
+    ),
     "tk_attn_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64]),
     "tk_attn_device_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int), _vp]),
     "tk_attn_set_wait_timeout_ns": (ctypes.c_int, [ctypes.c_ulonglong]),
