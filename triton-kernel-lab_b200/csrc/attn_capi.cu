@@ -121,6 +121,37 @@ int make_map_f32(CUtensorMap* map, const float* base, int64_t bh, int64_t seq, i
   return r == CUDA_SUCCESS ? tk::kOk : tk::kErrTensorMap;
 }
 
+// 4-D map over a strided (batch, heads, rows, D) 16-bit tensor (element
+// strides; those of dimensions of size 1 are not used): box {64, 128, 1, 1},
+// 128-byte swizzle, zero fill.
+int make_map_strided(CUtensorMap* map, const void* base, int64_t batch, int64_t heads, int64_t rows, int64_t head_dim,
+                     const int64_t* strides, int dtype) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return tk::kErrNoDriver;
+  const int64_t size[3] = {batch, heads, rows};
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(rows),
+                        static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(batch)};
+  cuuint64_t bytes[3];
+  for (int i = 0; i < 3; ++i) bytes[2 - i] = static_cast<cuuint64_t>(size[i] > 1 ? strides[i] : head_dim) * 2;
+  cuuint32_t box[4] = {64, 128, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, dtype == TK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                  const_cast<void*>(base), dims, bytes, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? tk::kOk : tk::kErrTensorMap;
+}
+
+// SMs of the current device; 0 without one.
+int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();  // do not leave the error for the next launch check
+    return 0;
+  }
+  return sms;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 }  // namespace
@@ -434,8 +465,13 @@ int tk_rotary(const void* q, const void* k, void* q_out, void* k_out, const floa
 
 size_t tk_tree_attn_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t nodes, int64_t seq_kv,
                                     int64_t head_dim) {
-  (void)batch, (void)q_heads, (void)kv_heads, (void)nodes, (void)seq_kv, (void)head_dim;
-  return 0;
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || nodes <= 0 || seq_kv <= 0 || head_dim <= 0 ||
+      q_heads % kv_heads != 0 || batch > (1 << 20) || q_heads > (1 << 20) || nodes > tk::kTreeMaxNodes ||
+      seq_kv > (1 << 30) || head_dim > 128)
+    return 0;
+  const int sms = sm_count();
+  if (sms <= 0) return 0;
+  return tk::tree_attn_workspace_bytes(batch, kv_heads, q_heads / kv_heads, nodes, seq_kv, head_dim, sms);
 }
 
 int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree, const void* v_tree,
@@ -452,7 +488,9 @@ int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree
   if (head_dim < 8 || head_dim > 128 || head_dim % 8 != 0 || nodes > tk::kTreeMaxNodes) return tk::kErrUnsupported;
   if (dtype != TK_DTYPE_F16 && dtype != TK_DTYPE_BF16) return tk::kErrUnsupported;
   if (!std::isfinite(scale) || scale <= 0.0f) return tk::kErrInvalidArgument;
-  if (seq_kv > (1 << 30) || batch > (1 << 20) || q_heads > (1 << 20) || batch * q_heads * nodes > (1 << 30))
+  // Key tiles and query rows are counted in 32 bits.
+  if (seq_kv > (1 << 30) || batch > (1 << 20) || q_heads > (1 << 20) || batch * q_heads * nodes > (1 << 30) ||
+      batch * kv_heads * ((seq_kv + 127) / 128 + 2) > (1 << 30))
     return tk::kErrTooLarge;
   for (const void* p : {q, k, v, k_tree, v_tree, static_cast<const void*>(o)})
     if (!aligned16(p)) return tk::kErrMisaligned;
@@ -460,18 +498,27 @@ int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree
                         static_cast<const void*>(tree_sizes), static_cast<const void*>(lse)})
     if (reinterpret_cast<uintptr_t>(p) & 3u) return tk::kErrMisaligned;
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return tk::kErrMisaligned;
-  if (workspace_bytes < tk_tree_attn_workspace_bytes(batch, q_heads, kv_heads, nodes, seq_kv, head_dim))
-    return tk::kErrInvalidArgument;
-  tk::TreeAttnArgs a{};
-  for (int i = 0; i < 12; ++i) {
+  for (int i = 0; i < 12; ++i)
     if (strides[i] < 0 || strides[i] % 8 != 0) return tk::kErrMisaligned;
-    a.strides[i] = strides[i];
-  }
-  a.q = q;
-  a.k = k;
-  a.v = v;
-  a.k_tree = k_tree;
-  a.v_tree = v_tree;
+  tk::TreeAttnArgs a{};
+  if (int rc = status_ptr(&a.status)) return rc;
+  a.sms = sm_count();
+  if (a.sms <= 0) return tk::kErrNoDriver;
+  const int64_t group = q_heads / kv_heads;
+  if (workspace == nullptr ||
+      workspace_bytes < tk::tree_attn_workspace_bytes(batch, kv_heads, group, nodes, seq_kv, head_dim, a.sms))
+    return tk::kErrInvalidArgument;
+  CUtensorMap mq, mk, mv, mkt, mvt;
+  if (int rc = make_map(&mq, q, batch * kv_heads, group * nodes, head_dim, dtype)) return rc;
+  if (int rc = make_map_strided(&mk, k, batch, kv_heads, seq_kv, head_dim, strides, dtype)) return rc;
+  if (int rc = make_map_strided(&mv, v, batch, kv_heads, seq_kv, head_dim, strides + 3, dtype)) return rc;
+  if (int rc = make_map_strided(&mkt, k_tree, batch, kv_heads, nodes, head_dim, strides + 6, dtype)) return rc;
+  if (int rc = make_map_strided(&mvt, v_tree, batch, kv_heads, nodes, head_dim, strides + 9, dtype)) return rc;
+  a.tm_q = &mq;
+  a.tm_k = &mk;
+  a.tm_v = &mv;
+  a.tm_kt = &mkt;
+  a.tm_vt = &mvt;
   a.kv_lens = kv_lens;
   a.parents = parents;
   a.tree_sizes = tree_sizes;
@@ -480,12 +527,14 @@ int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree
   a.parent_stride = parent_stride;
   a.B = batch;
   a.Hkv = kv_heads;
-  a.G = q_heads / kv_heads;
+  a.G = group;
   a.T = nodes;
   a.L = seq_kv;
   a.D = head_dim;
   a.bf16 = dtype == TK_DTYPE_BF16;
   a.scale_log2 = scale * kLog2e;
+  a.workspace = workspace;
+  a.timeout_ns = g_timeout_ns;
   a.stream = static_cast<cudaStream_t>(stream);
   return tk::launch_tree_attn(a);
 }

@@ -203,22 +203,27 @@ constexpr int kTreeMaxNodes = 256;
 
 // Tree attention over a cache (tree_attn_sm100.cu).
 struct TreeAttnArgs {
-  const void* q;       // (B, Hkv * G, T, D)
-  const void* k;       // cache (B, Hkv, L, D), strided
-  const void* v;
-  const void* k_tree;  // (B, Hkv, T, D), strided
-  const void* v_tree;
   const int* kv_lens;     // (B)
   const int* parents;     // (B or 1, T), or nullptr: a chain
   const int* tree_sizes;  // (B), or nullptr: T each
   void* o;                // (B, Hkv * G, T, D)
   float* lse;             // (B, Hkv * G, T), or nullptr
   int64_t parent_stride;  // T, or 0 for one tree shared by all sequences
-  int64_t strides[12];    // elements: k, v, k_tree, v_tree x (batch, head, row)
   int64_t B, Hkv, G, T, L, D;
   bool bf16;
   float scale_log2;
+  void* workspace;  // tree_attn_workspace_bytes
+  int sms;
+  unsigned long long timeout_ns;
+  int* status;
   cudaStream_t stream;
+  // q as (B Hkv, G T, D) with 128-row boxes; the caches and the tree's rows as
+  // (B, Hkv, rows, D) at their strides, 128-row boxes.
+  const CUtensorMap* tm_q;
+  const CUtensorMap* tm_k;
+  const CUtensorMap* tm_v;
+  const CUtensorMap* tm_kt;
+  const CUtensorMap* tm_vt;
 };
 
 // Verification of drafted tokens and the cache commit (speculative_sm100.cu).
@@ -258,6 +263,7 @@ struct CommitArgs {
 
 int launch_rotary(const RotaryArgs& a);
 int launch_tree_attn(const TreeAttnArgs& a);
+size_t tree_attn_workspace_bytes(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms);
 int launch_verify(const VerifyArgs& a);
 int launch_commit(const CommitArgs& a);
 int launch_attn_fwd(const FwdArgs& a);
