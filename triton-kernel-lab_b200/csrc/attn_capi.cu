@@ -490,7 +490,7 @@ int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree
   if (!std::isfinite(scale) || scale <= 0.0f) return tk::kErrInvalidArgument;
   // Key tiles and query rows are counted in 32 bits.
   if (seq_kv > (1 << 30) || batch > (1 << 20) || q_heads > (1 << 20) || batch * q_heads * nodes > (1 << 30) ||
-      batch * kv_heads * ((seq_kv + 127) / 128 + 2) > (1 << 30))
+      batch * kv_heads * ((seq_kv + 127) / 128 + 8) > (1 << 30))
     return tk::kErrTooLarge;
   for (const void* p : {q, k, v, k_tree, v_tree, static_cast<const void*>(o)})
     if (!aligned16(p)) return tk::kErrMisaligned;
@@ -509,7 +509,9 @@ int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree
       workspace_bytes < tk::tree_attn_workspace_bytes(batch, kv_heads, group, nodes, seq_kv, head_dim, a.sms))
     return tk::kErrInvalidArgument;
   CUtensorMap mq, mk, mv, mkt, mvt;
-  if (int rc = make_map(&mq, q, batch * kv_heads, group * nodes, head_dim, dtype)) return rc;
+  if (int rc = make_map(&mq, q, batch * kv_heads, group * nodes, head_dim, dtype,
+                        static_cast<uint32_t>(tk::tree_attn_q_box_rows(group, nodes))))
+    return rc;
   if (int rc = make_map_strided(&mk, k, batch, kv_heads, seq_kv, head_dim, strides, dtype)) return rc;
   if (int rc = make_map_strided(&mv, v, batch, kv_heads, seq_kv, head_dim, strides + 3, dtype)) return rc;
   if (int rc = make_map_strided(&mkt, k_tree, batch, kv_heads, nodes, head_dim, strides + 6, dtype)) return rc;

@@ -217,7 +217,7 @@ struct TreeAttnArgs {
   unsigned long long timeout_ns;
   int* status;
   cudaStream_t stream;
-  // q as (B Hkv, G T, D) with 128-row boxes; the caches and the tree's rows as
+  // q as (B Hkv, G T, D) with tree_attn_q_box_rows; the caches and the tree's rows as
   // (B, Hkv, rows, D) at their strides, 128-row boxes.
   const CUtensorMap* tm_q;
   const CUtensorMap* tm_k;
@@ -263,6 +263,8 @@ struct CommitArgs {
 
 int launch_rotary(const RotaryArgs& a);
 int launch_tree_attn(const TreeAttnArgs& a);
+// Box rows of the query map: 128, or the rows of one copy.
+int tree_attn_q_box_rows(int64_t G, int64_t T);
 size_t tree_attn_workspace_bytes(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms);
 int launch_verify(const VerifyArgs& a);
 int launch_commit(const CommitArgs& a);

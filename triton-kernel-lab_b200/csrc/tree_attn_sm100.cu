@@ -17,6 +17,13 @@
 // packed 16-bit pairs.  Keys of an item are its cache tiles, the last one cut
 // at kv_lens[b], then the tree's tiles under a bit per (row, node).
 //
+// With 64 rows or fewer the M rows are filled with kRep = 2 or 4 copies of
+// them: copy i's warps take the i-th part of every tile's keys, with a
+// running maximum, sum and O of their own (the other keys' P is zero there),
+// and the copies are joined through shared memory at the end of a segment.  A
+// row's softmax step then takes half or a quarter of the time, which bounds
+// short rows: one warp's 128 columns a row took about 3000 cycles a tile.
+//
 // Work is cut where the lengths are known, on the device: an item is a (batch,
 // KV head), its work its key tiles, and the items' tiles in one row are
 // divided into equal runs, one per CTA (of each group of 128 kT rows), so a
@@ -37,30 +44,45 @@
 namespace tk {
 namespace {
 
-// D: kernel width (64 or 128); kT: 128-row query tiles per CTA.
-template <int D, int kT>
+// D: kernel width (64 or 128); kT: 128-row query tiles per CTA; kRep: copies of
+// the rows in the one tile (1, 2 or 4).
+template <int D, int kT, int kRep>
 struct TreeCfg {
-  static constexpr int kThreads = 128 * (1 + kT);
-  static constexpr int kMinBlocks = D == 64 ? 2 : 1;
-  // S buffers per query tile: with one tile per CTA and SM a second one lets
-  // S(j + 1) run under the softmax of S(j); two CTAs or tiles cover each other.
-  static constexpr int kLook = (D == 128 && kT == 1) ? 2 : 1;
-  static constexpr int kStages = (kT == 1) ? 3 : 2;
+  static_assert(kRep == 1 || kT == 1, "copies fill one tile");
+  static constexpr int kMinBlocks = (D == 64 && kRep == 1) ? 2 : 1;
+  // One tile per CTA and SM: a warpgroup of its own for the epilogue and two
+  // O buffers, so a segment's end does not hold up the next one's tiles, and a
+  // second S buffer, so S(j + 1) runs under the softmax of S(j).  Two CTAs or
+  // two tiles cover each other instead.
+  static constexpr bool kEpi = kT == 1 && kMinBlocks == 1;
+  static constexpr int kLook = kEpi ? 2 : 1;
+  static constexpr int kThreads = 128 * (1 + kT + (kEpi ? 1 : 0));
+  // Stages of K and of V.
+  static constexpr int kStages = (D == 64 && kRep > 1) ? 5 : 3;
+  static constexpr int kVStages = (D == 64 && kRep > 1) ? 4 : (kT == 1 && kRep == 1) ? 3 : 2;
+  static constexpr int kQBufs = (D == 64 && kRep > 1) ? 2 : 1;
+  static constexpr int kRows = kT * kTileRows / kRep;  // query rows per CTA
   // 0: launched with registers to spare, no redistribution.
-  static constexpr int kLaunchRegs = (D == 64) ? 128 : (kT == 2 ? 168 : 0);
+  static constexpr int kLaunchRegs = (kMinBlocks == 2) ? 128 : (kRep == 1) ? 168 : 0;
   static constexpr int kRegsCtrl = 56;
-  static constexpr int kRegsSoftmax = (D == 64) ? 200 : 224;
-  static_assert(kLaunchRegs == 0 || kRegsCtrl + kT * kRegsSoftmax <= (1 + kT) * kLaunchRegs, "register split");
+  static constexpr int kRegsWork = (kMinBlocks == 2) ? 200 : 224;  // of the other warpgroups
+  static_assert(kLaunchRegs == 0 || kRegsCtrl + (kThreads / 128 - 1) * kRegsWork <= kThreads / 128 * kLaunchRegs,
+                "register split exceeds the launch");
   static constexpr int kTileBytes = kTileRows * D * 2;
-  static constexpr int kKOff = kT * kTileBytes;
+  static constexpr int kKOff = kQBufs * kT * kTileBytes;
   static constexpr int kVOff = kKOff + kStages * kTileBytes;
-  static constexpr int kBarOff = kVOff + kStages * kTileBytes;
-  // q_full, q_empty, k_full[S], k_empty[S], v_full[S], v_empty[S], s_full[2], p_ready[2], o_final[2], pv_done
-  static constexpr int kNumBars = 2 + 4 * kStages + 7;
+  static constexpr int kJoinOff = kVOff + kVStages * kTileBytes;
+  static constexpr int kJoinCols = 64;  // columns of O joined at a time (every copy, fp32)
+  static constexpr int kBarOff = kJoinOff + (kRep > 1 ? kTileRows * kJoinCols * 4 : 0);
+  // q_full[Q], q_empty[Q], k_full[S], k_empty[S], v_full[S], v_ok[S], v_empty[S], s_full[2], p_ready[2], o_final[2],
+  // o_empty[2], l_ready[2], pv_done
+  static constexpr int kNumBars = 2 * kQBufs + 2 * kStages + 3 * kVStages + 11;
   static constexpr int kCtlOff = kBarOff + kNumBars * 8;
-  static constexpr int kSmemBytes = kCtlOff + 16 + 32 + 64;  // control, first segment, scan
-  static constexpr uint32_t kTmemCols = (D == 64) ? 256 : 512;
-  static constexpr uint32_t kColS0 = kT * D;  // O of tile x at column x D, S buffers from here
+  static constexpr int kMlOff = (kCtlOff + 16 + 32 + 64 + 7) / 8 * 8;  // after control, first segment, scan
+  static constexpr int kSmemBytes = kMlOff + (kEpi ? 2 * kTileRows * 8 : 0);  // m and l of a segment's rows, two buffers
+  static constexpr uint32_t kTmemCols = (kMinBlocks == 2) ? 256 : 512;
+  // O of query tile x, or O buffer x, at column x D; the S buffers from here.
+  static constexpr uint32_t kColS0 = (kEpi ? 2 : kT) * D;
 };
 
 constexpr float kTreeRescale = 8.0f;  // as the forward's: P stays below 2^8, O is rescaled rarely
@@ -93,57 +115,75 @@ struct TreeSeg {
   int b, h, j0, j1, n_cache, n_all, len;
 };
 
-// Walks a CTA's run, one segment at a time.
+// What an item costs beyond its tiles (its query load, first scores and
+// epilogue), in tiles: runs are equal in tiles plus this, so that a CTA with
+// many short items gets fewer tiles.  Sequences of 0 to 4096 keys, 64 wide, 24
+// of them: with 0, the slowest CTA took 1.29 times the median's time.
+constexpr int kItemCost = 2;
+__device__ __forceinline__ int item_cost(const TreeShape& s, int b) {
+  return tiles_of(cache_len(s, b)) + tiles_of(s.T) + kItemCost;
+}
+
+// Walks a CTA's run, one segment at a time.  u: place in the item's cost, its
+// first kItemCost units holding no tile.
 struct TreeWalk {
-  int b, h, j, left;
+  int b, h, u, left;
   __device__ __forceinline__ bool next(const TreeShape& s, TreeSeg& seg) {
-    if (left <= 0) return false;
-    seg.b = b;
-    seg.h = h;
-    seg.len = cache_len(s, b);
-    seg.n_cache = tiles_of(seg.len);
-    seg.n_all = seg.n_cache + tiles_of(s.T);
-    seg.j0 = j;
-    seg.j1 = min(seg.n_all, j + left);
-    left -= seg.j1 - seg.j0;
-    j = 0;
-    if (++h == s.Hkv) {
-      h = 0;
-      ++b;
+    while (left > 0) {
+      seg.b = b;
+      seg.h = h;
+      seg.len = cache_len(s, b);
+      seg.n_cache = tiles_of(seg.len);
+      seg.n_all = seg.n_cache + tiles_of(s.T);
+      const int end = min(seg.n_all + kItemCost, u + left);
+      seg.j0 = max(u - kItemCost, 0);
+      seg.j1 = max(end - kItemCost, 0);
+      left -= end - u;
+      u = 0;
+      if (++h == s.Hkv) {
+        h = 0;
+        ++b;
+      }
+      if (seg.j1 > seg.j0) return true;
     }
-    return true;
+    return false;
   }
 };
 
-// The start of the workspace: the run length, then each batch's first tile
-// (of one KV head's worth: multiply by Hkv).
+// The start of the workspace, for the joining kernel: an entry per item or, if
+// there are fewer runs, per run, written by the CTA that begins the item: the
+// cut item (b Hkv + h, -1: none), the run of its first part, that part's slot
+// and the number of parts.
 struct TreePlan {
-  int* run;
-  int* base;
+  int4* cut;
+  int by_item;
 };
 
 // One 128-key tile of one row: as the forward's softmax step, with `mask`
-// (kMasked) a bit per key.
-template <bool kBf16, bool kMasked, int kEmuPairs>
-__device__ __forceinline__ void softmax_tile(uint32_t s_addr, const uint32_t (&mask)[4], float scale_log2, float& m_run,
-                                             float& l_run, float& alpha, bool& need) {
-  uint32_t s[4][32];
-  tmem_ld32(s_addr, s[0]);
-  tmem_ld32(s_addr + 32, s[1]);
+// (kMasked) a bit per key.  With copies (kRep > 1) only copy `copy`'s 128 /
+// kRep keys; P of the others is zero.
+template <bool kBf16, bool kMasked, int kEmuPairs, int kRep>
+__device__ __forceinline__ void softmax_tile(uint32_t s_addr, int copy, const uint32_t (&mask)[4 / kRep], float scale_log2,
+                                             float& m_run, float& l_run, float& alpha, bool& need) {
+  constexpr int kBlocks = 4 / kRep;  // 32-key blocks
+  uint32_t s[kBlocks][32];
+  const uint32_t own = s_addr + copy * (32 * kBlocks);
+#pragma unroll
+  for (int b = 0; b < (kBlocks + 1) / 2; ++b) tmem_ld32(own + 32 * b, s[b]);
   tmem_wait_ld();
-  reg_fence(s[0]);
-  reg_fence(s[1]);
-  tmem_ld32(s_addr + 64, s[2]);
-  tmem_ld32(s_addr + 96, s[3]);
+#pragma unroll
+  for (int b = 0; b < (kBlocks + 1) / 2; ++b) reg_fence(s[b]);
+#pragma unroll
+  for (int b = (kBlocks + 1) / 2; b < kBlocks; ++b) tmem_ld32(own + 32 * b, s[b]);
   float mx[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) mx[i] = -INFINITY;
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    if (b == 2) {
+  for (int b = 0; b < kBlocks; ++b) {
+    if (kBlocks > 1 && b == kBlocks / 2) {
       tmem_wait_ld();
-      reg_fence(s[2]);
-      reg_fence(s[3]);
+#pragma unroll
+      for (int i = kBlocks / 2; i < kBlocks; ++i) reg_fence(s[i]);
     }
 #pragma unroll
     for (int c = 0; c < 32; c += 2) {
@@ -164,8 +204,15 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, const uint32_t (&m
   const uint64_t scale2 = f2_pack(scale_log2, scale_log2);
   const uint64_t negm2 = f2_pack(-ms, -ms);
   uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+  if constexpr (kRep > 1) {
+    // S is in registers: zero P everywhere else.
+    const uint32_t zero[16] = {};
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
+    for (int b = 0; b < 4; ++b)
+      if (b / kBlocks != copy) tmem_st16(s_addr + b * 16, zero);
+  }
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
     uint32_t pk[16];
 #pragma unroll
     for (int c = 0; c < 32; c += 2) {
@@ -182,7 +229,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, const uint32_t (&m
       sum2[(c >> 1) & 1] = fadd2(sum2[(c >> 1) & 1], f2_pack(p0, p1));
       pk[c >> 1] = pack2<kBf16>(p0, p1);
     }
-    tmem_st16(s_addr + b * 16, pk);
+    tmem_st16(s_addr + (copy * kBlocks + b) * 16, pk);
   }
   float sa0, sa1, sb0, sb1;
   f2_unpack(sum2[0], sa0, sa1);
@@ -191,39 +238,185 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, const uint32_t (&m
   m_run = m_use;
 }
 
-// Bit n of the result: the row's node attends tree node 128 tile + n.
-__device__ __forceinline__ void tree_mask(const TreeShape& s, int b, int node, int size, int tile, uint32_t (&mask)[4]) {
+// The first n bits of W words (none below 0, all from 32 W on).
+template <int W>
+__device__ __forceinline__ void first_bits(int n, uint32_t (&mask)[W]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) mask[i] = 0;
+  for (int i = 0; i < W; ++i) {
+    const int k = n - 32 * i;
+    mask[i] = k >= 32 ? 0xffffffffu : k > 0 ? (1u << k) - 1u : 0u;
+  }
+}
+
+// Bit n of the W words: the row's node attends tree node lo + n.
+template <int W>
+__device__ __forceinline__ void tree_mask(const TreeShape& s, int b, int node, int size, int lo, uint32_t (&mask)[W]) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) mask[i] = 0;
   if (node >= size) return;
-  const int lo = tile * kTileRows;
   if (s.parents == nullptr) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = node + 1 - lo - 32 * i;  // nodes of this word up to and including the row's own
-      mask[i] = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
-    }
+    first_bits(node + 1 - lo, mask);
     return;
   }
   const int* up = s.parents + b * s.parent_stride;
   while (node >= lo) {  // ends: every step goes to a smaller node
     const int n = node - lo;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < W; ++i)
       if ((n >> 5) == i) mask[i] |= 1u << (n & 31);
     const int parent = up[node];
     node = parent < node ? parent : -1;
   }
 }
 
-template <int D, int kT, bool kBf16>
-__global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMinBlocks)
+// The end of a segment for one row held by one thread: O from tensor memory
+// to the output (whole items) or, unnormalised with m and l, to a part's row.
+template <int D, bool kBf16>
+__device__ __forceinline__ void finish_row(uint32_t o_addr, bool whole, bool live, bool row_ok, float m, float l,
+                                           long long row_g, long long prow, int d_real, uint16_t* out, float* lse,
+                                           float* part_ml, float* part_o) {
+  if (whole) {
+    const bool wide_store = (d_real % 16) == 0 && (reinterpret_cast<uintptr_t>(out) & 31u) == 0;
+    const float inv = (live && l > 0.0f) ? 1.0f / l : 0.0f;
+    uint16_t* orow = out + row_g * d_real;
+#pragma unroll
+    for (int cb = 0; cb < D / 32; ++cb) {
+      uint32_t o[32];
+      tmem_ld32(o_addr + cb * 32, o);
+      tmem_wait_ld();
+      reg_fence(o);
+      uint32_t w[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        w[e] = live ? pack2<kBf16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv) : 0u;
+      if (row_ok) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int col = cb * 32 + hh * 16;
+          if (wide_store && col < d_real) {
+            st_global_v8(orow + col, &w[hh * 8]);
+          } else if (!wide_store) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              if (col + q * 8 < d_real)
+                *reinterpret_cast<uint4*>(orow + col + q * 8) = make_uint4(
+                    w[hh * 8 + q * 4], w[hh * 8 + q * 4 + 1], w[hh * 8 + q * 4 + 2], w[hh * 8 + q * 4 + 3]);
+          }
+        }
+      }
+    }
+    if (lse != nullptr && row_ok) lse[row_g] = live ? m + lg2(l) : -INFINITY;
+  } else {
+#pragma unroll
+    for (int cb = 0; cb < D / 32; ++cb) {
+      uint32_t o[32];
+      tmem_ld32(o_addr + cb * 32, o);
+      tmem_wait_ld();
+      reg_fence(o);
+      if (!live) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0u;
+      }
+      if (row_ok) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) st_global_v8(part_o + prow * D + cb * 32 + q * 8, &o[q * 8]);
+      }
+    }
+    if (row_ok) *reinterpret_cast<float2*>(part_ml + prow * 2) = live ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+  }
+}
+
+// The end of a segment whose rows are held as kRep copies: thread r holds row
+// r % (128 / kRep) of copy r / (128 / kRep).  64 columns at a time, each row
+// weighted by 2^(m - M) goes to shared memory (16-byte chunks XORed with the
+// row), then kRep threads a row add the copies and store.  All 128 threads
+// call it; `ok` only skips the work.
+template <int D, int kRep, bool kBf16>
+__device__ __forceinline__ void finish_copies(bool ok, uint32_t o_addr, int r, bool whole, const float2* ml, float4* join,
+                                              int R, long long item_row, long long slot_row, int d_real, uint16_t* out,
+                                              float* lse, float* part_ml, float* part_o) {
+  constexpr int kCopyRows = kTileRows / kRep;
+  constexpr int kCols = 64 / kRep;
+  const int mrow = r % kCopyRows;  // the row it writes
+  const int jrow = r / kRep, jpart = r % kRep;  // the row and columns it finishes
+  float top = -INFINITY, jtop = -INFINITY, jl = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kRep; ++i) {
+    top = fmaxf(top, ml[i * kCopyRows + mrow].x);
+    jtop = fmaxf(jtop, ml[i * kCopyRows + jrow].x);
+  }
+  // Weight 0: a copy without keys, or rows that no warp computed.
+  const float w = ml[r].x == -INFINITY ? 0.0f : ex2(ml[r].x - top);
+#pragma unroll
+  for (int i = 0; i < kRep; ++i) {
+    const float2 e = ml[i * kCopyRows + jrow];
+    if (e.x != -INFINITY) jl += ex2(e.x - jtop) * e.y;
+  }
+  const float scale = whole ? (jl > 0.0f ? 1.0f / jl : 0.0f) : 1.0f;
+  const bool jrow_ok = ok && jrow < R;
+#pragma unroll
+  for (int pass = 0; pass < D / 64; ++pass) {
+    if (pass > 0) named_barrier_sync(1, 128);
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      uint32_t o[32];
+      if (ok) {
+        tmem_ld32(o_addr + pass * 64 + cb * 32, o);
+        tmem_wait_ld();
+        reg_fence(o);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        join[r * 16 + ((cb * 8 + q) ^ (r & 7))] =
+            w != 0.0f ? make_float4(w * __uint_as_float(o[4 * q]), w * __uint_as_float(o[4 * q + 1]),
+                                   w * __uint_as_float(o[4 * q + 2]), w * __uint_as_float(o[4 * q + 3]))
+                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    named_barrier_sync(1, 128);
+    if (!jrow_ok) continue;
+#pragma unroll
+    for (int c = 0; c < kCols; c += 8) {
+      float4 f[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        f[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < kRep; ++i) {
+          const int jr = i * kCopyRows + jrow;
+          const float4 g = join[jr * 16 + (((jpart * kCols + c) / 4 + q) ^ (jr & 7))];
+          f[q].x += g.x, f[q].y += g.y, f[q].z += g.z, f[q].w += g.w;
+        }
+      }
+      const int col = pass * 64 + jpart * kCols + c;
+      if (whole) {
+        if (col < d_real)
+          *reinterpret_cast<uint4*>(out + (item_row + jrow) * d_real + col) =
+              make_uint4(pack2<kBf16>(f[0].x * scale, f[0].y * scale), pack2<kBf16>(f[0].z * scale, f[0].w * scale),
+                         pack2<kBf16>(f[1].x * scale, f[1].y * scale), pack2<kBf16>(f[1].z * scale, f[1].w * scale));
+      } else {
+        float4* dst = reinterpret_cast<float4*>(part_o + (slot_row + jrow) * D + col);
+        dst[0] = f[0];
+        dst[1] = f[1];
+      }
+    }
+  }
+  if (jrow_ok && jpart == 0) {
+    if (!whole)
+      *reinterpret_cast<float2*>(part_ml + (slot_row + jrow) * 2) = make_float2(jtop, jl);
+    else if (lse != nullptr)
+      lse[item_row + jrow] = jl == 0.0f ? -INFINITY : jtop + lg2(jl);
+  }
+  named_barrier_sync(1, 128);  // before the next segment's ml and columns
+}
+
+template <int D, int kT, int kRep, bool kBf16>
+__global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, TreeCfg<D, kT, kRep>::kMinBlocks)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_kt,
                      const __grid_constant__ CUtensorMap tm_vt, const __grid_constant__ TreeShape shape,
                      uint16_t* __restrict__ out, float* __restrict__ lse, TreePlan plan, float* __restrict__ part_ml,
                      float* __restrict__ part_o, float scale_log2, unsigned long long timeout_ns, int* status) {
-  using C = TreeCfg<D, kT>;
+  using C = TreeCfg<D, kT, kRep>;
   constexpr int kLook = C::kLook;
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {
@@ -233,38 +426,48 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int wg = warp >> 2;
-  const int group = blockIdx.x;  // rows [group 128 kT, ...) of every item
+  const int group = blockIdx.x;  // rows [group kRows, ...) of every item
 
   uint8_t* sQ = smem;
   uint8_t* sK = smem + C::kKOff;
   uint8_t* sV = smem + C::kVOff;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  uint64_t* q_empty = q_full + 1;
-  uint64_t* k_full = q_empty + 1;
+  uint64_t* q_empty = q_full + C::kQBufs;
+  uint64_t* k_full = q_empty + C::kQBufs;
   uint64_t* k_empty = k_full + C::kStages;
   uint64_t* v_full = k_empty + C::kStages;
-  uint64_t* v_empty = v_full + C::kStages;
-  uint64_t* s_full = v_empty + C::kStages;  // [2]: query tile, or S buffer of the one tile
+  uint64_t* v_ok = v_full + C::kVStages;  // full, and cleared past the last valid key
+  uint64_t* v_empty = v_ok + C::kVStages;
+  uint64_t* s_full = v_empty + C::kVStages;  // [2]: query tile, or S buffer of the one tile
   uint64_t* p_ready = s_full + 2;           // [2]
-  uint64_t* o_final = p_ready + 2;          // [2]: query tile
-  uint64_t* pv_done = o_final + 2;          // with two S buffers: P V of every tile
+  uint64_t* o_final = p_ready + 2;          // [2]: query tile, or O buffer
+  uint64_t* o_empty = o_final + 2;          // [2]: O buffer read by the epilogue
+  uint64_t* l_ready = o_empty + 2;          // [2]: m and l of O buffer's segment written
+  uint64_t* pv_done = l_ready + 2;          // with two S buffers: P V of every tile
   CtaControl* ctl = reinterpret_cast<CtaControl*>(smem + C::kCtlOff);
-  int* first = reinterpret_cast<int*>(smem + C::kCtlOff + 16);  // b, h, j, tiles of this CTA's run
+  int* first = reinterpret_cast<int*>(smem + C::kCtlOff + 16);  // this CTA's run: b, h, u, length; the runs' length
   int* scan = first + 8;                                         // [warps]
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    for (int i = 0; i < C::kQBufs; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < C::kVStages; ++i) {
       mbar_init(&v_full[i], 1);
+      mbar_init(&v_ok[i], 1);
       mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 4);
       mbar_init(&o_final[i], 1);
+      mbar_init(&o_empty[i], 4);
+      mbar_init(&l_ready[i], 4);
     }
     mbar_init(pv_done, 1);
     ctl->abort = 0;
@@ -279,13 +482,12 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
   }
   if (warp == 1) tmem_alloc(&ctl->tmem_base, C::kTmemCols);
 
-  // This CTA's run: a scan of the batch's tiles, each thread over consecutive sequences.
+  // This CTA's run: a scan of the batch's costs, each thread over consecutive sequences.
   {
     const int per = (shape.B + C::kThreads - 1) / C::kThreads;
     const int b0 = min(static_cast<int>(threadIdx.x) * per, shape.B), b1 = min(b0 + per, shape.B);
-    const int tree_tiles = tiles_of(shape.T);
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += tiles_of(cache_len(shape, b)) + tree_tiles;
+    for (int b = b0; b < b1; ++b) mine += item_cost(shape, b);
     int upto = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -304,18 +506,18 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
     total *= shape.Hkv;
     const int run = (total + gridDim.y - 1) / gridDim.y;
     const int start = blockIdx.y * run;
-    if (threadIdx.x == 0) first[3] = max(min(run, total - start), 0);
-    const bool writes = blockIdx.x == 0 && blockIdx.y == 0;
-    if (writes && threadIdx.x == 0) *plan.run = run;
+    if (threadIdx.x == 0) {
+      first[3] = max(min(run, total - start), 0);
+      first[4] = run;
+    }
     for (int b = b0; b < b1; ++b) {
-      const int n = tiles_of(cache_len(shape, b)) + tree_tiles;
+      const int n = item_cost(shape, b);
       const int from = before * shape.Hkv;
       if (start >= from && start < from + n * shape.Hkv) {
         first[0] = b;
         first[1] = (start - from) / n;
         first[2] = (start - from) % n;
       }
-      if (writes) plan.base[b] = before;
       before += n;
     }
   }
@@ -331,7 +533,7 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
   if (wg == 0) {
     if constexpr (C::kLaunchRegs != 0) warpgroup_reg_dec<C::kRegsCtrl>();
     if (warp == 0 || warp == 2) {
-      // ---------------- TMA producers: warp 0 Q and K, warp 2 V ----------------
+      // ---------------- TMA producers: warp 0 K, warp 2 V ----------------
       if (lane == 0) {
         const bool is_k = warp == 0;
         uint8_t* ring = is_k ? sK : sV;
@@ -339,20 +541,11 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
         uint64_t* empty = is_k ? k_empty : v_empty;
         uint32_t g = 0;
         bool ok = true;
-        for (int it = 0; ok && walk.next(shape, seg); ++it) {
-          if (is_k) {
-            if (it > 0 && !(ok = mbar_wait(q_empty, (it - 1) & 1, ctl, timeout_ns, status, 1))) break;
-            mbar_arrive_expect_tx(q_full, kT * C::kTileBytes);
-#pragma unroll
-            for (int x = 0; x < kT; ++x)
-#pragma unroll
-              for (int blk = 0; blk < D / 64; ++blk)
-                tma_load_3d(sQ + x * C::kTileBytes + blk * kBlockBytes, &tm_q, q_full, blk * 64,
-                            (group * kT + x) * kTileRows, seg.b * shape.Hkv + seg.h);
-          }
+        while (ok && walk.next(shape, seg)) {
           for (int j = seg.j0; j < seg.j1; ++j, ++g) {
-            const int st = g % C::kStages;
-            if (!(ok = mbar_wait(&empty[st], ((g / C::kStages) & 1) ^ 1, ctl, timeout_ns, status, is_k ? 2 : 3))) break;
+            const uint32_t depth = is_k ? C::kStages : C::kVStages;
+            const int st = g % depth;
+            if (!(ok = mbar_wait(&empty[st], ((g / depth) & 1) ^ 1, ctl, timeout_ns, status, is_k ? 2 : 3))) break;
             mbar_arrive_expect_tx(&full[st], C::kTileBytes);
             const bool on_cache = j < seg.n_cache;
             const CUtensorMap* map = on_cache ? (is_k ? &tm_k : &tm_v) : (is_k ? &tm_kt : &tm_vt);
@@ -363,6 +556,59 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
           }
         }
       }
+    } else if (warp == 3) {
+      // ---------------- Q, the tails of V, and the joining kernel's entries ----------------
+      int4 mine = make_int4(-1, 0, 0, 0);
+      uint32_t g = 0;
+      bool ok = true;
+      for (int it = 0; ok && walk.next(shape, seg); ++it) {
+        const int qb = it % C::kQBufs;
+        if (it >= C::kQBufs &&
+            !(ok = warp_wait(&q_empty[qb], ((it / C::kQBufs) & 1) ^ 1, ctl, timeout_ns, status, 1)))
+          break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&q_full[qb], kT * C::kTileBytes);
+          // kT tiles of 128 rows, or kRep copies of 128 / kRep.
+#pragma unroll
+          for (int x = 0; x < kT * kRep; ++x)
+#pragma unroll
+            for (int blk = 0; blk < D / 64; ++blk)
+              tma_load_3d(sQ + (qb * kT + x / kRep) * C::kTileBytes + blk * kBlockBytes +
+                              (x % kRep) * (kTileRows / kRep) * kSwizzleBytes,
+                          &tm_q, &q_full[qb], blk * 64, group * C::kRows + (kRep == 1 ? x * kTileRows : 0),
+                          seg.b * shape.Hkv + seg.h);
+          if (group == 0 && seg.j0 == 0) {
+            const bool cut = seg.j1 < seg.n_all;
+            const int item = seg.b * shape.Hkv + seg.h;
+            const int4 e = cut ? make_int4(item, blockIdx.y, it > 0 ? 1 : 0,
+                                           1 + (seg.n_all - seg.j1 + first[4] - 1) / first[4])
+                               : make_int4(-1, 0, 0, 0);
+            if (plan.by_item)
+              plan.cut[item] = e;
+            else if (cut)
+              mine = e;
+          }
+        }
+        const int size = tree_size(shape, seg.b);
+        for (int j = seg.j0; j < seg.j1; ++j, ++g) {
+          const int st = g % C::kVStages;
+          if (!(ok = warp_wait(&v_full[st], (g / C::kVStages) & 1, ctl, timeout_ns, status, 15))) break;
+          // Rows of V past the last valid key: cleared.
+          const int jt = j - seg.n_cache;
+          const int valid = jt < 0 ? seg.len - j * kTileRows : size - jt * kTileRows;
+          if (valid < kTileRows) {
+            const int from = max(valid, 0) * kSwizzleBytes;
+#pragma unroll
+            for (int blk = 0; blk < D / 64; ++blk)
+              for (int off = from + lane * 16; off < kBlockBytes; off += 32 * 16)
+                *reinterpret_cast<uint4*>(sV + st * C::kTileBytes + blk * kBlockBytes + off) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&v_ok[st]);
+        }
+      }
+      if (lane == 0 && group == 0 && !plan.by_item) plan.cut[blockIdx.y] = mine;
     } else if (warp == 1) {
       // ---------------- MMA issuer ----------------
       const bool leader = elect_one();
@@ -373,8 +619,8 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
       const uint32_t v_lo0 = sdesc_lo_mnmajor(smem_u32(sV), kTileRows);
       constexpr uint32_t kTileLo = C::kTileBytes >> 4;
       // Query tile x (kT = 2), or S buffer x of the one tile.
-      auto issue_s = [&](int x, int st) {
-        const uint32_t q_lo = q_lo0 + (kT == 2 ? x * kTileLo : 0u);
+      auto issue_s = [&](int x, int qb, int st) {
+        const uint32_t q_lo = q_lo0 + (kT == 2 ? x : qb) * kTileLo;
         const uint32_t k_lo = k_lo0 + st * kTileLo;
         if (leader) {
 #pragma unroll
@@ -385,9 +631,9 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
         }
         __syncwarp();
       };
-      auto issue_pv = [&](int x, int st, bool accumulate) {
+      auto issue_pv = [&](int x, int ob, int st, bool accumulate) {
         const uint32_t v_lo = v_lo0 + st * kTileLo;
-        const uint32_t d = tmem + (kT == 2 ? D * x : 0u);
+        const uint32_t d = tmem + (kT == 2 ? D * x : D * ob);
         if (leader) {
 #pragma unroll
           for (int kk = 0; kk < kTileRows / 16; ++kk)
@@ -404,61 +650,53 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
       bool ok = true;
       for (int it = 0; ok && walk.next(shape, seg); ++it) {
         const int n = seg.j1 - seg.j0;
-        const int size = tree_size(shape, seg.b);
+        const int qb = it % C::kQBufs;
+        const int ob = C::kEpi ? it & 1 : 0;  // O buffer
         // S of tile i of the segment (every query tile), with what it frees.
         auto scores = [&](int i) -> bool {
           const int st = (g + i) % C::kStages;
           if (!warp_wait(&k_full[st], ((g + i) / C::kStages) & 1, ctl, timeout_ns, status, 4)) return false;
           tc_fence_after();
-          if constexpr (kT == 1) issue_s((g + i) % kLook, st);
+          if constexpr (kT == 1) issue_s((g + i) % kLook, qb, st);
           return true;
         };
         auto scores_done = [&](int i) {
           commit(&k_empty[(g + i) % C::kStages]);
-          if (i == n - 1) commit(q_empty);
+          if (i == n - 1) commit(&q_empty[qb]);
         };
-        if (!(ok = warp_wait(q_full, it & 1, ctl, timeout_ns, status, 5))) break;
+        if (!(ok = warp_wait(&q_full[qb], (it / C::kQBufs) & 1, ctl, timeout_ns, status, 5))) break;
         for (int i = 0; i < min(kLook, n); ++i) {
           if (!(ok = scores(i))) break;
           if constexpr (kT == 2) {
-            issue_s(0, g % C::kStages);
-            issue_s(1, g % C::kStages);
+            issue_s(0, 0, g % C::kStages);
+            issue_s(1, 0, g % C::kStages);
           }
           scores_done(i);
         }
         for (int j = 0; ok && j < n; ++j) {
           const uint32_t gj = g + j;
-          const int st = gj % C::kStages;
+          const int st = gj % C::kVStages;
 #pragma unroll
           for (int x = 0; x < kT; ++x) {
             const int buf = kT == 2 ? x : static_cast<int>(gj % kLook);
             if (!(ok = warp_wait(&p_ready[buf], (gj / kLook) & 1, ctl, timeout_ns, status, 6))) break;
             if (x == 0) {
-              if (!(ok = warp_wait(&v_full[st], (gj / C::kStages) & 1, ctl, timeout_ns, status, 7))) break;
-              // Rows of V past the last valid key: cleared.
-              const int jt = seg.j0 + j - seg.n_cache;
-              const int valid = jt < 0 ? seg.len - (seg.j0 + j) * kTileRows : size - jt * kTileRows;
-              if (valid < kTileRows) {
-                const int from = max(valid, 0) * kSwizzleBytes;
-#pragma unroll
-                for (int blk = 0; blk < D / 64; ++blk)
-                  for (int off = from + lane * 16; off < kBlockBytes; off += 32 * 16)
-                    *reinterpret_cast<uint4*>(sV + st * C::kTileBytes + blk * kBlockBytes + off) = make_uint4(0, 0, 0, 0);
-                fence_proxy_async_smem();
-                __syncwarp();
-              }
+              if (!(ok = warp_wait(&v_ok[st], (gj / C::kVStages) & 1, ctl, timeout_ns, status, 7))) break;
+            }
+            if (C::kEpi && j == 0 && it >= 2) {
+              if (!(ok = warp_wait(&o_empty[ob], ((it >> 1) & 1) ^ 1, ctl, timeout_ns, status, 11))) break;
             }
             tc_fence_after();
-            issue_pv(buf, st, j > 0);
+            issue_pv(buf, ob, st, j > 0);
             if (x == kT - 1) commit(&v_empty[st]);
             if constexpr (kLook == 2) commit(pv_done);
-            if (j == n - 1) commit(&o_final[x]);
+            if (j == n - 1) commit(&o_final[C::kEpi ? ob : x]);
             if (j + kLook < n) {
               if constexpr (kT == 1) {
                 if (!(ok = scores(j + kLook))) break;
               } else {
                 if (x == 0 && !(ok = scores(j + 1))) break;
-                issue_s(x, (gj + 1) % C::kStages);
+                issue_s(x, 0, (gj + 1) % C::kStages);
               }
               if (x == kT - 1) scores_done(j + kLook);
             }
@@ -467,46 +705,43 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
         g += n;
       }
     }
-  } else {
-    if constexpr (C::kLaunchRegs != 0) warpgroup_reg_inc<C::kRegsSoftmax>();
-    // ---------------- softmax, correction and epilogue of query tile x ----------------
+  } else if (wg <= kT) {
+    if constexpr (C::kLaunchRegs != 0) warpgroup_reg_inc<C::kRegsWork>();
+    // ---------------- softmax and correction of query tile x (and its epilogue) ----------------
     const int x = wg - 1;
     const int q4 = warp & 3;
     const int r = q4 * 32 + lane;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
-    const uint32_t o_addr = t_lane + D * x;
-    const int row = (group * kT + x) * kTileRows + r;  // of the item's R rows
+    constexpr int kCopyRows = kTileRows / kRep;
+    const int copy = r / kCopyRows;
+    const int row = group * C::kRows + x * kTileRows + r % kCopyRows;  // of the item's R rows
     const int node = row % shape.T;
     const bool any_row = row - lane < shape.R;  // some row of this warp exists
-    const bool wide_store = (shape.d_real % 16) == 0 && (reinterpret_cast<uintptr_t>(out) & 31u) == 0;
     uint32_t g = 0;
     bool ok = true;
     for (int it = 0; ok && walk.next(shape, seg); ++it) {
+      const uint32_t o_addr = t_lane + D * (C::kEpi ? it & 1 : x);
       const int size = tree_size(shape, seg.b);
       float m_run = -INFINITY, l_run = 0.0f;
       for (int j = seg.j0; ok && j < seg.j1; ++j, ++g) {
         const int buf = kT == 2 ? x : static_cast<int>(g % kLook);
         const uint32_t s_addr = t_lane + C::kColS0 + 128u * buf;
-        uint32_t mask[4];
+        uint32_t mask[4 / kRep];
         const bool on_tree = j >= seg.n_cache;
         const int lim = seg.len - j * kTileRows;
-        if (on_tree) tree_mask(shape, seg.b, row < shape.R ? node : size, size, j - seg.n_cache, mask);
+        if (on_tree)
+          tree_mask(shape, seg.b, row < shape.R ? node : size, size, (j - seg.n_cache) * kTileRows + copy * kCopyRows, mask);
         if (!(ok = warp_wait(&s_full[buf], (g / kLook) & 1, ctl, timeout_ns, status, 8))) break;
         tc_fence_after();
         if (any_row) {
           float alpha;
           bool need;
           if (on_tree || lim < kTileRows) {
-            if (!on_tree) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int n = lim - 32 * i;
-                mask[i] = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
-              }
-            }
-            softmax_tile<kBf16, true, 0>(s_addr, mask, scale_log2, m_run, l_run, alpha, need);
+            if (!on_tree) first_bits(lim - copy * kCopyRows, mask);
+            softmax_tile<kBf16, true, 0, kRep>(s_addr, copy, mask, scale_log2, m_run, l_run, alpha, need);
           } else {
-            softmax_tile<kBf16, false, kLook == 2 ? 0 : 3>(s_addr, mask, scale_log2, m_run, l_run, alpha, need);
+            softmax_tile<kBf16, false, kLook == 2 ? 0 : 3, kRep>(s_addr, copy, mask, scale_log2, m_run, l_run, alpha,
+                                                                 need);
           }
           // O may be rescaled once P V of the tile before is in it: with one S
           // buffer S(j) completing says so.
@@ -532,70 +767,65 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[buf]);
       }
-      if (ok) ok = warp_wait(&o_final[x], it & 1, ctl, timeout_ns, status, 10);
-      if (!ok || !any_row) continue;
-      tc_fence_after();
-      const bool whole = seg.j0 == 0 && seg.j1 == seg.n_all;
+      if (!ok) break;
       const bool live = node < size;  // other rows: nothing
-      const bool row_ok = row < shape.R;
-      const long long row_g = (static_cast<long long>(seg.b) * shape.Hkv + seg.h) * shape.R + row;
-      if (whole) {
-        const float inv = (live && l_run > 0.0f) ? 1.0f / l_run : 0.0f;
-        uint16_t* orow = out + row_g * shape.d_real;
-#pragma unroll
-        for (int cb = 0; cb < D / 32; ++cb) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + cb * 32, o);
-          tmem_wait_ld();
-          reg_fence(o);
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            w[e] = live ? pack2<kBf16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv) : 0u;
-          if (row_ok) {
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              const int col = cb * 32 + hh * 16;
-              if (wide_store && col < shape.d_real) {
-                st_global_v8(orow + col, &w[hh * 8]);
-              } else if (!wide_store) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-                  if (col + q * 8 < shape.d_real)
-                    *reinterpret_cast<uint4*>(orow + col + q * 8) = make_uint4(
-                        w[hh * 8 + q * 4], w[hh * 8 + q * 4 + 1], w[hh * 8 + q * 4 + 2], w[hh * 8 + q * 4 + 3]);
-              }
-            }
-          }
-        }
-        if (lse != nullptr && row_ok) lse[row_g] = live ? m_run + lg2(l_run) : -INFINITY;
+      if constexpr (C::kEpi) {
+        const int ob = it & 1;
+        if (it >= 2 && !(ok = warp_wait(&o_empty[ob], ((it >> 1) & 1) ^ 1, ctl, timeout_ns, status, 12))) break;
+        if (l_run != l_run) m_run = 0.0f;  // a NaN row stays one
+        reinterpret_cast<float2*>(smem + C::kMlOff)[ob * kTileRows + r] =
+            (any_row && live) ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.0f);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&l_ready[ob]);
       } else {
-        // A part: unnormalised O, m and l.  Slot 0 of this CTA for its first segment, 1 for its last.
-        const long long slot = (static_cast<long long>(blockIdx.y) * gridDim.x + group) * 2 + (it > 0 ? 1 : 0);
-        const long long prow = slot * (kT * kTileRows) + x * kTileRows + r;
-#pragma unroll
-        for (int cb = 0; cb < D / 32; ++cb) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + cb * 32, o);
-          tmem_wait_ld();
-          reg_fence(o);
-          if (!live) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
-          }
-          if (row_ok) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) st_global_v8(part_o + prow * D + cb * 32 + q * 8, &o[q * 8]);
-          }
-        }
-        if (row_ok)
-          *reinterpret_cast<float2*>(part_ml + prow * 2) = live ? make_float2(m_run, l_run) : make_float2(-INFINITY, 0.0f);
+        if (!(ok = warp_wait(&o_final[x], it & 1, ctl, timeout_ns, status, 10))) break;
+        if (!any_row) continue;
+        tc_fence_after();
+        const long long slot_row =
+            ((static_cast<long long>(blockIdx.y) * gridDim.x + group) * 2 + (it > 0 ? 1 : 0)) * C::kRows;
+        finish_row<D, kBf16>(o_addr, seg.j0 == 0 && seg.j1 == seg.n_all, live, row < shape.R, m_run, l_run,
+                             (static_cast<long long>(seg.b) * shape.Hkv + seg.h) * shape.R + row,
+                             slot_row + x * kTileRows + r, shape.d_real, out, lse, part_ml, part_o);
       }
     }
+  } else {
+    if constexpr (C::kLaunchRegs != 0) warpgroup_reg_inc<C::kRegsWork>();
+    // ---------------- epilogue (kEpi) ----------------
+    const int q4 = warp & 3;
+    const int r = q4 * 32 + lane;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
+    bool ok = true;
+    // (Every warp walks every segment, failed or not: the copies meet at
+    // barriers.)
+    for (int it = 0; walk.next(shape, seg); ++it) {
+      const int ob = it & 1;
+      if (ok) ok = warp_wait(&l_ready[ob], (it >> 1) & 1, ctl, timeout_ns, status, 13);
+      if (ok) ok = warp_wait(&o_final[ob], (it >> 1) & 1, ctl, timeout_ns, status, 14);
+      if (ok) tc_fence_after();
+      const bool whole = seg.j0 == 0 && seg.j1 == seg.n_all;
+      const long long item_row = (static_cast<long long>(seg.b) * shape.Hkv + seg.h) * shape.R;
+      // A part's slot: 0 of this CTA for its first segment, 1 for its last.
+      const long long slot_row =
+          ((static_cast<long long>(blockIdx.y) * gridDim.x + group) * 2 + (it > 0 ? 1 : 0)) * C::kRows;
+      const float2* ml = reinterpret_cast<const float2*>(smem + C::kMlOff) + ob * kTileRows;
+      if constexpr (kRep > 1) {
+        finish_copies<D, kRep, kBf16>(ok, t_lane + D * ob, r, whole, ml, reinterpret_cast<float4*>(smem + C::kJoinOff),
+                                      shape.R, item_row, slot_row, shape.d_real, out, lse, part_ml, part_o);
+      } else if (ok && group * C::kRows + r - lane < shape.R) {
+        const int row = group * C::kRows + r;
+        finish_row<D, kBf16>(t_lane + D * ob, whole, ml[r].y != 0.0f, row < shape.R, ml[r].x, ml[r].y, item_row + row,
+                             slot_row + r, shape.d_real, out, lse, part_ml, part_o);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_empty[ob]);
+    }
   }
-  pdl_launch_dependents();
   tc_fence_before();
   __syncthreads();
+  // Now, not earlier: blocks of the joining kernel would sit on SMs where
+  // this grid still works.
+  pdl_launch_dependents();
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -605,153 +835,188 @@ __global__ void __launch_bounds__(TreeCfg<D, kT>::kThreads, TreeCfg<D, kT>::kMin
 
 constexpr int kJoinWarps = 8;
 
-// Joins the parts of the rows whose item was cut: with M the largest m,
-// o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over its parts in run
-// order.  warps_per_row warps (1 to 8) share a row's parts.
-template <int D, bool kBf16>
+// Joins the parts of cut items: with M the largest m,
+// o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over a row's parts in run
+// order.  Bound by the latency of the loads (a row's parts are a few KB, in
+// L2), so each warp keeps eight rows of parts in flight: kRows rows with
+// 8 / kRows parts each, or one row whose parts kShare warps divide.
+template <int D, bool kBf16, int kRows, int kShare>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     tree_attn_combine_kernel(const __grid_constant__ TreeShape shape, uint16_t* __restrict__ out,
                              float* __restrict__ lse, TreePlan plan, const float* __restrict__ part_ml,
-                             const float* __restrict__ part_o, int groups, int group_rows, int warps_per_row) {
+                             const float* __restrict__ part_o, int groups, int group_rows) {
+  static_assert(kRows == 1 || kShare == 1, "rows of a warp, or warps of a row");
   constexpr int kPer = D / 32;
-  __shared__ float s_acc[kJoinWarps][D];
-  __shared__ float s_ml[kJoinWarps][2];
+  constexpr int kBatch = 8 / kRows;
   pdl_wait_prerequisites();
+  const int4 cut = plan.cut[blockIdx.y];
+  if (cut.x < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int share = warp % warps_per_row;
-  const long long row_g = static_cast<long long>(blockIdx.x) * (kJoinWarps / warps_per_row) + warp / warps_per_row;
-  const bool exists = row_g < static_cast<long long>(shape.B) * shape.Hkv * shape.R;
-  int c0 = 0, c1 = 0, start = 0, row = 0;
-  const int run = *plan.run;
-  if (exists) {
-    row = static_cast<int>(row_g % shape.R);
-    const int item = static_cast<int>(row_g / shape.R);
-    const int b = item / shape.Hkv, h = item % shape.Hkv;
-    const int n = tiles_of(cache_len(shape, b)) + tiles_of(shape.T);
-    start = plan.base[b] * shape.Hkv + h * n;
-    c0 = start / run;
-    c1 = (start + n - 1) / run;
-  }
-  const bool cut = c1 > c0;
-  float acc[kPer], m = -INFINITY, l = 0.0f;
+  const int share = warp % kShare;
+  const int row0 = (blockIdx.x * (kJoinWarps / kShare) + warp / kShare) * kRows;
+  float acc[kRows][kPer], m[kRows], l[kRows];
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
-  if (cut) {
-    const int group = row / group_rows;
-    constexpr int kBatch = 8;  // parts loaded before any is used
-    for (int c = c0 + share; c <= c1; c += warps_per_row * kBatch) {
-      float2 ml[kBatch];
-      float v[kBatch][kPer];
+  for (int k = 0; k < kRows; ++k) {
+    m[k] = -INFINITY;
+    l[k] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[k][e] = 0.0f;
+  }
+  for (int p = share; p < cut.w; p += kShare * kBatch) {
+    float2 ml[kRows][kBatch];
+    float v[kRows][kBatch][kPer];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int row = row0 + k;
+      const int group = row / group_rows;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int ci = c + i * warps_per_row;
-        ml[i] = make_float2(-INFINITY, 0.0f);
+        const int pi = p + i * kShare;
+        ml[k][i] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) v[i][e] = 0.0f;
-        if (ci <= c1) {
-          const long long slot = (static_cast<long long>(ci) * groups + group) * 2 + (static_cast<long long>(ci) * run >= start ? 0 : 1);
+        for (int e = 0; e < kPer; ++e) v[k][i][e] = 0.0f;
+        if (pi < cut.w && row < shape.R) {
+          const long long slot = (static_cast<long long>(cut.y + pi) * groups + group) * 2 + (pi == 0 ? cut.z : 0);
           const long long prow = slot * group_rows + row % group_rows;
-          ml[i] = *reinterpret_cast<const float2*>(part_ml + prow * 2);
+          ml[k][i] = *reinterpret_cast<const float2*>(part_ml + prow * 2);
           const float* src = part_o + prow * D + lane * kPer;
           if constexpr (kPer == 4) {
             const float4 q = *reinterpret_cast<const float4*>(src);
-            v[i][0] = q.x, v[i][1] = q.y, v[i][2] = q.z, v[i][3] = q.w;
+            v[k][i][0] = q.x, v[k][i][1] = q.y, v[k][i][2] = q.z, v[k][i][3] = q.w;
           } else {
             const float2 q = *reinterpret_cast<const float2*>(src);
-            v[i][0] = q.x, v[i][1] = q.y;
+            v[k][i][0] = q.x, v[k][i][1] = q.y;
           }
         }
       }
-      float top = m;
+    }
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[i].x);
+    for (int k = 0; k < kRows; ++k) {
+      float top = m[k];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[k][i].x);
       if (top == -INFINITY) continue;
-      const float keep = ex2(m - top);
-      m = top;
-      l *= keep;
+      const float keep = ex2(m[k] - top);
+      m[k] = top;
+      l[k] *= keep;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) acc[e] *= keep;
+      for (int e = 0; e < kPer; ++e) acc[k][e] *= keep;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const float w = ex2(ml[i].x - top);
-        l += w * ml[i].y;
+        const float w = ex2(ml[k][i].x - top);
+        l[k] += w * ml[k][i].y;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] += w * v[i][e];
+        for (int e = 0; e < kPer; ++e) acc[k][e] += w * v[k][i][e];
       }
     }
   }
-  if (warps_per_row > 1) {
+  if constexpr (kShare > 1) {
+    __shared__ float s_acc[kJoinWarps][D];
+    __shared__ float s_ml[kJoinWarps][2];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) s_acc[warp][lane * kPer + e] = acc[e];
+    for (int e = 0; e < kPer; ++e) s_acc[warp][lane * kPer + e] = acc[0][e];
     if (lane == 0) {
-      s_ml[warp][0] = m;
-      s_ml[warp][1] = l;
+      s_ml[warp][0] = m[0];
+      s_ml[warp][1] = l[0];
     }
     __syncthreads();
     if (share != 0) return;
     float top = -INFINITY;
-    for (int i = 0; i < warps_per_row; ++i) top = fmaxf(top, s_ml[warp + i][0]);
-    m = top;
-    l = 0.0f;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
-    for (int i = 0; i < warps_per_row && top != -INFINITY; ++i) {
-      const float w = ex2(s_ml[warp + i][0] - top);
-      l += w * s_ml[warp + i][1];
+    for (int i = 0; i < kShare; ++i) top = fmaxf(top, s_ml[warp + i][0]);
+    m[0] = top;
+    l[0] = 0.0f;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) acc[e] += w * s_acc[warp + i][lane * kPer + e];
+    for (int e = 0; e < kPer; ++e) acc[0][e] = 0.0f;
+    if (top != -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < kShare; ++i) {
+        const float w = ex2(s_ml[warp + i][0] - top);
+        l[0] += w * s_ml[warp + i][1];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) acc[0][e] += w * s_acc[warp + i][lane * kPer + e];
+      }
     }
   }
-  if (!cut) return;
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  if (lane * kPer < shape.d_real) {
-    uint16_t* dst = out + row_g * shape.d_real + lane * kPer;
-    if constexpr (kPer == 4) {
-      *reinterpret_cast<uint2*>(dst) =
-          make_uint2(pack2<kBf16>(acc[0] * inv, acc[1] * inv), pack2<kBf16>(acc[2] * inv, acc[3] * inv));
-    } else {
-      *reinterpret_cast<uint32_t*>(dst) = pack2<kBf16>(acc[0] * inv, acc[1] * inv);
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    const int row = row0 + k;
+    if (row >= shape.R) continue;
+    const long long row_g = static_cast<long long>(cut.x) * shape.R + row;
+    const float inv = l[k] > 0.0f ? 1.0f / l[k] : 0.0f;
+    if (lane * kPer < shape.d_real) {
+      uint16_t* dst = out + row_g * shape.d_real + lane * kPer;
+      if constexpr (kPer == 4) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBf16>(acc[k][0] * inv, acc[k][1] * inv),
+                                                    pack2<kBf16>(acc[k][2] * inv, acc[k][3] * inv));
+      } else {
+        *reinterpret_cast<uint32_t*>(dst) = pack2<kBf16>(acc[k][0] * inv, acc[k][1] * inv);
+      }
     }
+    if (lse != nullptr && lane == 0) lse[row_g] = l[k] == 0.0f ? -INFINITY : m[k] + lg2(l[k]);
   }
-  if (lse != nullptr && lane == 0) lse[row_g] = l > 0.0f ? m + lg2(l) : -INFINITY;
 }
 
-// The launch: groups of 128 kT rows x runs, as many CTAs as are resident
-// together (or as there are key tiles at full caches, if fewer).
+// The launch: groups of kRows rows x runs, as many CTAs as are resident
+// together (or as the items cost at full caches, if less).
 struct TreeGrid {
   int groups, runs;
+  int cuts;  // entries of the plan: items or runs, whichever are fewer
   size_t plan_bytes, ml_bytes, o_bytes;
 };
 
 constexpr int tree_tiles_per_cta(int64_t D, int64_t R) { return D > 64 && R > kTileRows ? 2 : 1; }
+constexpr int tree_copies(int64_t R) { return R <= 32 ? 4 : R <= 64 ? 2 : 1; }
 
 TreeGrid tree_grid(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms) {
-  const int kT = tree_tiles_per_cta(D, G * T);
+  const int64_t group_rows = tree_tiles_per_cta(D, G * T) * kTileRows / tree_copies(G * T);
   const int64_t width = D > 64 ? 128 : 64;
-  const int64_t resident = sms * (width == 64 ? 2 : 1);
+  const int64_t resident = sms * (width == 64 && tree_copies(G * T) == 1 ? 2 : 1);
   TreeGrid t;
-  const int64_t groups = (G * T + kT * kTileRows - 1) / (kT * kTileRows);
-  const int64_t tiles = B * Hkv * ((L + kTileRows - 1) / kTileRows + (T + kTileRows - 1) / kTileRows);
+  const int64_t groups = (G * T + group_rows - 1) / group_rows;
+  const int64_t tiles = B * Hkv * ((L + kTileRows - 1) / kTileRows + (T + kTileRows - 1) / kTileRows + kItemCost);
   t.groups = static_cast<int>(groups);
   t.runs = static_cast<int>(std::max<int64_t>(1, std::min(resident / groups, tiles)));
-  const size_t rows = static_cast<size_t>(groups) * t.runs * 2 * kT * kTileRows;
-  t.plan_bytes = (256 + static_cast<size_t>(B) * 4 + 255) / 256 * 256;
+  const size_t rows = static_cast<size_t>(groups) * t.runs * 2 * group_rows;
+  t.cuts = static_cast<int>(std::min<int64_t>(B * Hkv, t.runs));
+  t.plan_bytes = (static_cast<size_t>(t.cuts) * sizeof(int4) + 255) / 256 * 256;
   t.ml_bytes = rows * 8;
   t.o_bytes = rows * static_cast<size_t>(width) * 4;
   return t;
 }
 
-template <int D, int kT, bool kBf16>
+template <int D, bool kBf16, int kRows, int kShare>
+int launch_tree_combine(const TreeAttnArgs& a, const TreeGrid& t, const TreeShape& shape, const TreePlan& plan,
+                        const float* part_ml, const float* part_o, int group_rows) {
+  const int64_t per_block = kJoinWarps / kShare * kRows;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((a.G * a.T + per_block - 1) / per_block), static_cast<unsigned>(t.cuts));
+  cfg.blockDim = dim3(32 * kJoinWarps);
+  cfg.stream = a.stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, tree_attn_combine_kernel<D, kBf16, kRows, kShare>, shape, static_cast<uint16_t*>(a.o),
+                         a.lse, plan, part_ml, part_o, t.groups, group_rows) != cudaSuccess) {
+    cudaGetLastError();
+    return kErrLaunch;
+  }
+  return kOk;
+}
+
+template <int D, int kT, int kRep, bool kBf16>
 int launch_tree_t(const TreeAttnArgs& a, const TreeGrid& t) {
-  using C = TreeCfg<D, kT>;
+  using C = TreeCfg<D, kT, kRep>;
   static_assert(C::kSmemBytes + 1024 <= 233472 / C::kMinBlocks, "shared memory exceeds the SM's");
-  auto kern = tree_attn_kernel<D, kT, kBf16>;
+  auto kern = tree_attn_kernel<D, kT, kRep, kBf16>;
   if (int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::kSmemBytes, C::kLaunchRegs, nullptr)) return rc;
   const TreeShape shape{a.kv_lens, a.tree_sizes, a.parents, a.parent_stride, static_cast<int>(a.B),
                         static_cast<int>(a.Hkv), static_cast<int>(a.T), static_cast<int>(a.L),
                         static_cast<int>(a.G * a.T), static_cast<int>(a.D)};
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
-  const TreePlan plan{reinterpret_cast<int*>(ws), reinterpret_cast<int*>(ws + 256)};
+  const TreePlan plan{reinterpret_cast<int4*>(ws), a.B * a.Hkv <= t.runs ? 1 : 0};
   float* part_ml = reinterpret_cast<float*>(ws + t.plan_bytes);
   float* part_o = reinterpret_cast<float*>(ws + t.plan_bytes + t.ml_bytes);
   const dim3 grid(static_cast<unsigned>(t.groups), static_cast<unsigned>(t.runs));
@@ -760,38 +1025,30 @@ int launch_tree_t(const TreeAttnArgs& a, const TreeGrid& t) {
                                                       a.scale_log2, a.timeout_ns, a.status);
   if (cudaGetLastError() != cudaSuccess) return kErrLaunch;
   if (t.runs == 1) return kOk;  // nothing is cut
-  const int64_t rows = a.B * a.Hkv * a.G * a.T;
-  // Few rows: several warps share a row's parts.
-  int warps_per_row = kJoinWarps;
-  while (warps_per_row > 1 && rows * warps_per_row > 148 * 32) warps_per_row /= 2;
-  const int64_t per_block = kJoinWarps / warps_per_row;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((rows + per_block - 1) / per_block));
-  cfg.blockDim = dim3(32 * kJoinWarps);
-  cfg.stream = a.stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, tree_attn_combine_kernel<D, kBf16>, shape, static_cast<uint16_t*>(a.o),
-                                             a.lse, plan, static_cast<const float*>(part_ml),
-                                             static_cast<const float*>(part_o), t.groups, kT * kTileRows, warps_per_row);
-  if (err != cudaSuccess) {
-    cudaGetLastError();
-    return kErrLaunch;
-  }
-  return kOk;
+  // An item has about runs / items parts and one: with four or more, warps
+  // share a row's parts.
+  const int64_t parts = t.runs / (a.B * a.Hkv);
+  if (parts >= 16) return launch_tree_combine<D, kBf16, 1, 8>(a, t, shape, plan, part_ml, part_o, C::kRows);
+  if (parts >= 4) return launch_tree_combine<D, kBf16, 1, 2>(a, t, shape, plan, part_ml, part_o, C::kRows);
+  return launch_tree_combine<D, kBf16, 4, 1>(a, t, shape, plan, part_ml, part_o, C::kRows);
 }
 
-template <bool kBf16>
-int launch_tree_b(const TreeAttnArgs& a, const TreeGrid& t) {
-  if (a.D <= 64) return launch_tree_t<64, 1, kBf16>(a, t);
-  if (tree_tiles_per_cta(a.D, a.G * a.T) == 1) return launch_tree_t<128, 1, kBf16>(a, t);
-  return launch_tree_t<128, 2, kBf16>(a, t);
+template <int D, bool kBf16>
+int launch_tree_r(const TreeAttnArgs& a, const TreeGrid& t) {
+  switch (tree_copies(a.G * a.T)) {
+    case 4: return launch_tree_t<D, 1, 4, kBf16>(a, t);
+    case 2: return launch_tree_t<D, 1, 2, kBf16>(a, t);
+    default: break;
+  }
+  if constexpr (D == 128) {
+    if (tree_tiles_per_cta(a.D, a.G * a.T) == 2) return launch_tree_t<128, 2, 1, kBf16>(a, t);
+  }
+  return launch_tree_t<D, 1, 1, kBf16>(a, t);
 }
 
 }  // namespace
+
+int tree_attn_q_box_rows(int64_t G, int64_t T) { return kTileRows / tree_copies(G * T); }
 
 size_t tree_attn_workspace_bytes(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms) {
   const TreeGrid t = tree_grid(B, Hkv, G, T, L, D, sms);
@@ -800,7 +1057,8 @@ size_t tree_attn_workspace_bytes(int64_t B, int64_t Hkv, int64_t G, int64_t T, i
 
 int launch_tree_attn(const TreeAttnArgs& a) {
   const TreeGrid t = tree_grid(a.B, a.Hkv, a.G, a.T, a.L, a.D, a.sms);
-  return a.bf16 ? launch_tree_b<true>(a, t) : launch_tree_b<false>(a, t);
+  if (a.D <= 64) return a.bf16 ? launch_tree_r<64, true>(a, t) : launch_tree_r<64, false>(a, t);
+  return a.bf16 ? launch_tree_r<128, true>(a, t) : launch_tree_r<128, false>(a, t);
 }
 
 }  // namespace tk
