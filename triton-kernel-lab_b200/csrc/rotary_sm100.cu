@@ -10,11 +10,26 @@
 // columns from r on are copied.  The backward is the transpose: the sine's
 // sign changes (`transpose`).  Long-context scalings (and their factor on the
 // tables) live in the tables, so they need nothing here.
+//
+// Bound by memory: 4 bytes an element and three operations.  A row's angles
+// are fp32 and serve every head, so a thread keeps those of its columns and
+// goes over the heads with them: loading them per head would be twice the
+// data.  A thread has two chunks of W columns, the two sides of its pairs in
+// the half layout, neighbours in the interleaved one or among the copied
+// columns; four heads of loads are in flight before the first is used.
+#include <algorithm>
+
 #include "attn_launch.h"
 #include "rope_sm100.cuh"
 
 namespace tk {
 namespace {
+
+// W 16-bit elements as they are loaded and stored.
+template <int W>
+struct alignas(2 * W) Chunk {
+  uint16_t e[W];
+};
 
 template <bool kBf16>
 __device__ __forceinline__ float from16(uint16_t h) {
@@ -34,62 +49,154 @@ __device__ __forceinline__ uint16_t to16(float x) {
   }
 }
 
-// One thread per column pair or copied column of one row.
-template <bool kBf16>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
-  const int half = a.rotary_dim / 2;
-  const int units = half + a.D - a.rotary_dim;  // pairs, then copied columns
-  const long long n = static_cast<long long>(a.B) * (a.Hq + a.Hkv) * a.S * units;
-  const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
-  for (long long u = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; u < n; u += stride) {
-    const int unit = static_cast<int>(u % units);
-    long long row = u / units;
-    const int s = static_cast<int>(row % a.S);
-    row /= a.S;
-    int h = static_cast<int>(row % (a.Hq + a.Hkv));
-    const long long b = row / (a.Hq + a.Hkv);
-    const bool is_q = h < a.Hq;
-    if (!is_q) h -= static_cast<int>(a.Hq);
-    const int64_t* st = is_q ? a.q_stride : a.k_stride;
-    const uint16_t* x = static_cast<const uint16_t*>(is_q ? a.q : a.k) + b * st[0] + h * st[1] + s * st[2];
-    uint16_t* y = static_cast<uint16_t*>(is_q ? a.q_out : a.k_out) + ((b * (is_q ? a.Hq : a.Hkv) + h) * a.S + s) * a.D;
-    if (unit >= half) {
-      const int c = a.rotary_dim + unit - half;
-      y[c] = x[c];
-      continue;
-    }
+constexpr int kRotaryThreads = 256;
+constexpr int kRotaryHeads = 4;  // heads in flight
+
+template <bool kBf16, bool kInterleaved, int W>
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryArgs a, int units, int heads_per_block) {
+  using C = Chunk<W>;
+  const int chunks = static_cast<int>(a.D) / W, turned = static_cast<int>(a.rotary_dim) / W;
+  const long long u = static_cast<long long>(blockIdx.x) * kRotaryThreads + threadIdx.x;
+  const long long tok = u / units;  // (b, s)
+  if (tok >= a.B * a.S) return;
+  const int unit = static_cast<int>(u - tok * units);
+  const long long b = tok / a.S, s = tok - b * a.S;
+  // The thread's chunks; the second may not exist (an odd number of copied ones).
+  int c1, c2;
+  bool turn1, turn2;
+  if constexpr (kInterleaved) {
+    c1 = 2 * unit;
+    c2 = c1 + 1;
+    turn1 = c1 < turned;
+    turn2 = c2 < turned;
+  } else {
+    const int pairs = turned / 2;
+    turn1 = turn2 = unit < pairs;
+    c1 = turn1 ? unit : turned + 2 * (unit - pairs);
+    c2 = turn1 ? unit + pairs : c1 + 1;
+  }
+  const bool has2 = c2 < chunks;
+  // Angles of this thread's pairs: W of them (half: the chunks' columns;
+  // interleaved: W / 2 a chunk).
+  float cs[W], sn[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
+  if (turn1) {
     long long pos = s;
     if (a.positions != nullptr)
-      pos = a.positions_64 ? static_cast<const long long*>(a.positions)[b * a.S + s]
-                           : static_cast<const int*>(a.positions)[b * a.S + s];
-    const int c1 = a.interleaved ? 2 * unit : unit;
-    const int c2 = a.interleaved ? c1 + 1 : unit + half;
+      pos = a.positions_64 ? static_cast<const long long*>(a.positions)[tok] : static_cast<const int*>(a.positions)[tok];
     if (pos < 0 || pos >= a.table_rows) {
       // No table row: report it, leave the row as it is.
       atomicCAS(a.status, kOk, kErrInvalidArgument);
-      y[c1] = x[c1];
-      y[c2] = x[c2];
-      continue;
+      turn1 = turn2 = false;
+    } else {
+      const long long t = pos * (a.rotary_dim / 2) + (kInterleaved ? c1 * (W / 2) : c1 * W);
+      if constexpr (W == 8) {  // rows of a multiple of 4 angles: t is one too
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+          if (kInterleaved && i > 0 && !turn2) break;
+          const float4 c = *reinterpret_cast<const float4*>(a.cos + t + i);
+          const float4 v = *reinterpret_cast<const float4*>(a.sin + t + i);
+          cs[i] = c.x, cs[i + 1] = c.y, cs[i + 2] = c.z, cs[i + 3] = c.w;
+          sn[i] = v.x, sn[i + 1] = v.y, sn[i + 2] = v.z, sn[i + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          if (kInterleaved && i >= W / 2 && !turn2) break;
+          cs[i] = a.cos[t + i];
+          sn[i] = a.sin[t + i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < W; ++i) sn[i] = a.transpose ? -sn[i] : sn[i];
     }
-    const float cs = a.cos[pos * half + unit];
-    const float sn = a.transpose ? -a.sin[pos * half + unit] : a.sin[pos * half + unit];
-    const float x1 = from16<kBf16>(x[c1]), x2 = from16<kBf16>(x[c2]);
-    y[c1] = to16<kBf16>(x1 * cs - x2 * sn);
-    y[c2] = to16<kBf16>(x2 * cs + x1 * sn);
   }
+  const int heads = static_cast<int>(a.Hq + a.Hkv);
+  const int h_end = min(heads, static_cast<int>(blockIdx.y + 1) * heads_per_block);
+  for (int h0 = blockIdx.y * heads_per_block; h0 < h_end; h0 += kRotaryHeads) {
+    C x1[kRotaryHeads], x2[kRotaryHeads];
+#pragma unroll
+    for (int i = 0; i < kRotaryHeads; ++i) {
+      const int h = h0 + i;
+      if (h >= h_end) break;
+      const bool is_q = h < a.Hq;
+      const int64_t* st = is_q ? a.q_stride : a.k_stride;
+      const uint16_t* x = static_cast<const uint16_t*>(is_q ? a.q : a.k) + b * st[0] +
+                          (is_q ? h : h - a.Hq) * st[1] + s * st[2];
+      x1[i] = *reinterpret_cast<const C*>(x + c1 * W);
+      if (has2) x2[i] = *reinterpret_cast<const C*>(x + c2 * W);
+    }
+#pragma unroll
+    for (int i = 0; i < kRotaryHeads; ++i) {
+      const int h = h0 + i;
+      if (h >= h_end) break;
+      C y1 = x1[i], y2 = x2[i];
+      if constexpr (kInterleaved) {
+#pragma unroll
+        for (int e = 0; e < W; e += 2) {
+          const float p = from16<kBf16>(x1[i].e[e]), q = from16<kBf16>(x1[i].e[e + 1]);
+          const float v = from16<kBf16>(x2[i].e[e]), w = from16<kBf16>(x2[i].e[e + 1]);
+          const int k = e / 2, l = W / 2 + e / 2;
+          if (turn1) {
+            y1.e[e] = to16<kBf16>(p * cs[k] - q * sn[k]);
+            y1.e[e + 1] = to16<kBf16>(q * cs[k] + p * sn[k]);
+          }
+          if (turn2) {
+            y2.e[e] = to16<kBf16>(v * cs[l] - w * sn[l]);
+            y2.e[e + 1] = to16<kBf16>(w * cs[l] + v * sn[l]);
+          }
+        }
+      } else if (turn1) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const float p = from16<kBf16>(x1[i].e[e]), q = from16<kBf16>(x2[i].e[e]);
+          y1.e[e] = to16<kBf16>(p * cs[e] - q * sn[e]);
+          y2.e[e] = to16<kBf16>(q * cs[e] + p * sn[e]);
+        }
+      }
+      const bool is_q = h < a.Hq;
+      uint16_t* y = static_cast<uint16_t*>(is_q ? a.q_out : a.k_out) +
+                    ((is_q ? b * a.Hq + h : b * a.Hkv + (h - a.Hq)) * a.S + s) * a.D;
+      *reinterpret_cast<C*>(y + c1 * W) = y1;
+      if (has2) *reinterpret_cast<C*>(y + c2 * W) = y2;
+    }
+  }
+}
+
+template <bool kBf16, bool kInterleaved, int W>
+int launch_rotary_w(const RotaryArgs& a) {
+  const int64_t chunks = a.D / W, turned = a.rotary_dim / W;
+  const int64_t units = kInterleaved ? (chunks + 1) / 2 : turned / 2 + (chunks - turned + 1) / 2;
+  const int64_t heads = a.Hq + a.Hkv;
+  const int64_t blocks = (a.B * a.S * units + kRotaryThreads - 1) / kRotaryThreads;
+  if (blocks > INT32_MAX) return kErrTooLarge;
+  // All heads in one thread where that fills the device (8 CTAs an SM are
+  // resident), else as few as it takes: short calls are bound by latency.
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>((heads + kRotaryHeads - 1) / kRotaryHeads, 148 * 8 / blocks));
+  const int64_t per = (heads + want - 1) / want;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((heads + per - 1) / per));
+  rotary_kernel<kBf16, kInterleaved, W><<<grid, kRotaryThreads, 0, a.stream>>>(a, static_cast<int>(units), static_cast<int>(per));
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+}
+
+// The widest chunk that rotated columns divide into: 16 bytes for the usual
+// widths, down to one column for pairs like (i, i + 3).
+template <bool kBf16>
+int launch_rotary_b(const RotaryArgs& a) {
+  if (a.interleaved) {
+    if (a.rotary_dim % 8 == 0) return launch_rotary_w<kBf16, true, 8>(a);
+    if (a.rotary_dim % 4 == 0) return launch_rotary_w<kBf16, true, 4>(a);
+    return launch_rotary_w<kBf16, true, 2>(a);
+  }
+  if (a.rotary_dim % 16 == 0) return launch_rotary_w<kBf16, false, 8>(a);
+  if (a.rotary_dim % 8 == 0) return launch_rotary_w<kBf16, false, 4>(a);
+  if (a.rotary_dim % 4 == 0) return launch_rotary_w<kBf16, false, 2>(a);
+  return launch_rotary_w<kBf16, false, 1>(a);
 }
 
 }  // namespace
 
-int launch_rotary(const RotaryArgs& a) {
-  const long long n = static_cast<long long>(a.B) * (a.Hq + a.Hkv) * a.S * (a.D - a.rotary_dim / 2);
-  const long long blocks = (n + 255) / 256;
-  const unsigned grid = static_cast<unsigned>(blocks < 148LL * 64 ? blocks : 148LL * 64);
-  if (a.bf16)
-    rotary_kernel<true><<<grid, 256, 0, a.stream>>>(a);
-  else
-    rotary_kernel<false><<<grid, 256, 0, a.stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
-}
+int launch_rotary(const RotaryArgs& a) { return a.bf16 ? launch_rotary_b<true>(a) : launch_rotary_b<false>(a); }
 
 }  // namespace tk

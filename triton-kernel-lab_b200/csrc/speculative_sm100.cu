@@ -40,79 +40,160 @@ __device__ __forceinline__ long long token_at(const VerifyArgs& a, int64_t i) {
   return a.tokens_64 ? static_cast<const long long*>(a.tokens)[i] : static_cast<const int*>(a.tokens)[i];
 }
 
-constexpr int kVerifyThreads = 1024;
+// Two scores of the race in one order: the larger score, then the lower
+// index (positive floats order like their bits); 0 is no token.
+__device__ __forceinline__ unsigned long long race_key(float score, int v) {
+  return (static_cast<unsigned long long>(__float_as_uint(score)) << 32) | (0xffffffffu - static_cast<unsigned>(v));
+}
 
-// One CTA per sequence.
-template <int kType>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
-  __shared__ int s_parent[kTreeMaxNodes], s_child[kTreeMaxNodes];
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+  unsigned n;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+// Every thread of every CTA of the cluster; sync orders shared-memory accesses.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void store_remote(const void* mine, unsigned rank, unsigned long long x) {
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\tst.shared::cluster.u64 [r], %2;\n\t}" ::"r"(
+          smem_u32(mine)),
+      "r"(rank), "l"(x)
+      : "memory");
+}
+
+constexpr int kVerifyThreads = 512;
+constexpr int kVerifyMaxCluster = 8;
+
+// N consecutive probabilities (or noise values), fp32; vector loads at N = 4.
+template <int kType, int N>
+__device__ __forceinline__ void load_probs(const void* p, int64_t i, float (&f)[N]) {
+  if constexpr (N == 1) {
+    f[0] = prob_at<kType>(p, i);
+  } else if constexpr (kType == kProbF32) {
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    const uint32_t u[2] = {v.x, v.y};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if constexpr (kType == kProbBf16) {
+        f[2 * k] = __uint_as_float(u[k] << 16);
+        f[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+      } else {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+        f[2 * k] = h.x;
+        f[2 * k + 1] = h.y;
+      }
+    }
+  }
+}
+
+// One cluster per sequence, its CTAs over the vocabulary.  Every CTA of it
+// walks the tree for itself (a few loads; sharing the result would cost a
+// cluster barrier more).  Bound by the row of p (and q) and the noise where
+// there are many sequences, by the chain of dependent loads (tokens, their
+// probabilities, the row) where there are few: the noise, which depends on
+// none, is brought into L2 meanwhile.
+//
+// The race divides only where it may win: w / e rounds to more than `best`
+// only if w > best e (1 - 2^-23), tested with a margin, so nearly every
+// element costs a multiplication and a comparison.
+template <int kType, int N>
+__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_constant__ VerifyArgs a) {
+  __shared__ int s_parent[kTreeMaxNodes], s_child[kTreeMaxNodes], s_path[kTreeMaxNodes];
   __shared__ long long s_token[kTreeMaxNodes];
-  __shared__ float s_prob[kTreeMaxNodes];
+  __shared__ float s_prob[kTreeMaxNodes], s_left[kTreeMaxNodes];
   __shared__ unsigned char s_pass[kTreeMaxNodes];
-  __shared__ int s_last;
-  __shared__ float s_score[32];
-  __shared__ int s_index[32];
-  const int64_t b = blockIdx.x;
+  __shared__ int s_last, s_length, s_tried;
+  __shared__ unsigned long long s_warp[kVerifyThreads / 32], s_best[2][kVerifyMaxCluster];
+  cluster_arrive();  // waited for before the first store to another CTA's shared memory
+  const unsigned rank = cluster_rank(), ranks = cluster_size();
+  const int64_t b = blockIdx.x / ranks;
   const int T = static_cast<int>(a.T), V = static_cast<int>(a.V);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // This CTA's part of the vocabulary, in steps of N.
+  const int steps = (V + N - 1) / N, per = (steps + ranks - 1) / ranks;
+  const int first = min(static_cast<int>(rank) * per, steps), end = min(first + per, steps);
+  const float* noise = a.noise + b * V;
+  for (int64_t i = static_cast<int64_t>(first) * N + threadIdx.x * 32; i < static_cast<int64_t>(end) * N; i += kVerifyThreads * 32)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + i));
+
   const int size = a.tree_sizes != nullptr ? min(max(a.tree_sizes[b], 0), T) : T;
-  for (int c = threadIdx.x; c < T; c += blockDim.x) {
+  for (int c = threadIdx.x; c < T; c += kVerifyThreads) {
     int n = c - 1;
     if (a.parents != nullptr && c > 0) n = a.parents[b * a.parent_stride + c];
     if (n >= c || n < 0 || c >= size) n = -1;  // hangs on nothing: never reached
     const long long x = token_at(a, b * T + c);
     const bool real = n >= 0 && x >= 0 && x < V;
+    const float p = real ? prob_at<kType>(a.target, b * a.target_stride[0] + n * a.target_stride[1] + x) : 0.0f;
+    bool pass = false;
+    if (a.draft != nullptr && p > 0.0f)
+      pass = a.uniforms[b * T + c] * prob_at<kType>(a.draft, b * a.draft_stride[0] + n * a.draft_stride[1] + x) < p;
     s_parent[c] = n;
     s_token[c] = x;
-    s_prob[c] = real ? prob_at<kType>(a.target, b * a.target_stride[0] + n * a.target_stride[1] + x) : 0.0f;
+    s_prob[c] = p;
+    s_pass[c] = pass;
     s_child[c] = -1;
   }
+  if (threadIdx.x == 0) s_tried = 0;
   __syncthreads();
-  for (int c = threadIdx.x; c < T; c += blockDim.x) {
-    bool pass = false;
-    const int n = s_parent[c];
-    if (n >= 0 && s_prob[c] > 0.0f) {
-      const float u = a.uniforms[b * T + c];
-      if (a.draft != nullptr) {
-        const float q = prob_at<kType>(a.draft, b * a.draft_stride[0] + n * a.draft_stride[1] + s_token[c]);
-        pass = u * q < s_prob[c];
-      } else {
-        float mass = 0.0f;
-        bool again = false;
-        for (int s = n + 1; s < c; ++s) {
-          if (s_parent[s] != n) continue;
-          if (s_token[s] == s_token[c]) again = true;
-          bool first = true;
-          for (int r = n + 1; r < s; ++r) first = first && !(s_parent[r] == n && s_token[r] == s_token[s]);
-          if (first) mass += s_prob[s];
-        }
-        pass = !again && u * fmaxf(1.0f - mass, 0.0f) < s_prob[c];
-      }
+  if (a.draft == nullptr) {
+    // A warp per node.  Its token's mass, unless an earlier sibling tried it ...
+    for (int c = warp; c < size; c += kVerifyThreads / 32) {
+      const int n = s_parent[c];
+      bool again = false;
+      if (n >= 0)
+        for (int s = n + 1 + lane; s < c; s += 32) again = again || (s_parent[s] == n && s_token[s] == s_token[c]);
+      again = __any_sync(0xffffffffu, again);
+      if (lane == 0) s_left[c] = again || !(s_prob[c] > 0.0f) ? 0.0f : s_prob[c];
     }
-    s_pass[c] = pass;
+    __syncthreads();
+    // ... against what its earlier siblings left.
+    for (int c = warp; c < size; c += kVerifyThreads / 32) {
+      const int n = s_parent[c];
+      float mass = 0.0f;
+      if (n >= 0)
+        for (int s = n + 1 + lane; s < c; s += 32) mass += s_parent[s] == n ? s_left[s] : 0.0f;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, off);
+      if (lane == 0 && n >= 0)
+        s_pass[c] = s_left[c] > 0.0f && a.uniforms[b * T + c] * fmaxf(1.0f - mass, 0.0f) < s_left[c];
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  for (int c = threadIdx.x; c < T; c += blockDim.x) {
-    if (!s_pass[c]) continue;
-    const int n = s_parent[c];
-    bool first = true;
-    for (int s = n + 1; s < c; ++s) first = first && !(s_parent[s] == n && s_pass[s]);
-    if (first) s_child[n] = c;
-  }
+  for (int c = threadIdx.x; c < size; c += kVerifyThreads)
+    if (s_pass[c]) {
+      const int n = s_parent[c];
+      bool lead = true;
+      for (int s = n + 1; s < c; ++s) lead = lead && !(s_parent[s] == n && s_pass[s]);
+      if (lead) s_child[n] = c;
+    }
   __syncthreads();
   if (threadIdx.x == 0) {
-    int last = -1, length = 0;
-    for (int n = size > 0 ? 0 : -1; n >= 0; n = s_child[n]) {
-      a.path[b * T + length++] = n;
-      last = n;
-    }
-    a.path_lens[b] = length;
-    for (int i = length; i < T; ++i) a.path[b * T + i] = -1;
-    s_last = last;
+    int length = 0;
+    for (int n = size > 0 ? 0 : -1; n >= 0; n = s_child[n]) s_path[length++] = n;
+    s_length = length;
+    s_last = length > 0 ? s_path[length - 1] : -1;
   }
   __syncthreads();
-  const int last = s_last;
-  if (last < 0) {
-    if (threadIdx.x == 0) {
+  cluster_wait();
+  const int last = s_last, length = s_length;
+  if (rank == 0) {
+    for (int i = threadIdx.x; i < T; i += kVerifyThreads) a.path[b * T + i] = i < length ? s_path[i] : -1;
+    if (threadIdx.x == 0) a.path_lens[b] = length;
+  }
+  if (last < 0) {  // the same in every CTA of the cluster
+    if (rank == 0 && threadIdx.x == 0) {
       if (a.tokens_64)
         static_cast<long long*>(a.next)[b] = -1;
       else
@@ -120,108 +201,187 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
     }
     return;
   }
-  bool has_child = false;
-  for (int c = last + 1; c < size; ++c) has_child = has_child || s_parent[c] == last;
+  // The tokens tried at the last node (s_token's first entries from here on).
+  __syncthreads();
+  if (warp == 0) {
+    int tried = 0;
+    for (int c0 = last + 1; c0 < size; c0 += 32) {
+      const int c = c0 + lane;
+      const bool mine = c < size && s_parent[c] == last;
+      const long long x = mine ? s_token[c] : 0;
+      const unsigned all = __ballot_sync(0xffffffffu, mine);
+      if (mine) s_token[tried + __popc(all & ((1u << lane) - 1u))] = x;
+      tried += __popc(all);
+      __syncwarp();
+    }
+    if (lane == 0) s_tried = tried;
+  }
+  __syncthreads();
+  const int tried = s_tried;
   const int64_t row = b * a.target_stride[0] + last * a.target_stride[1];
   const int64_t drow = a.draft != nullptr ? b * a.draft_stride[0] + last * a.draft_stride[1] : 0;
   for (int attempt = 0; attempt < 2; ++attempt) {
-    const bool residual = attempt == 0 && has_child;
-    float best = 0.0f;
-    int index = INT_MAX;
-    for (int v = threadIdx.x; v < V; v += blockDim.x) {
-      float w = prob_at<kType>(a.target, row + v);
-      if (residual) {
-        if (a.draft != nullptr) {
-          w -= prob_at<kType>(a.draft, drow + v);
-        } else {
-          for (int c = last + 1; c < size; ++c)
-            if (s_parent[c] == last && s_token[c] == v) w = 0.0f;
+    const bool residual = attempt == 0 && tried > 0;
+    const bool minus = residual && a.draft != nullptr;
+    float best = 0.0f, bar = 0.0f;
+    int index = 0;
+    constexpr int kFlight = 16 / N / (N > 1 ? 2 : 1);  // steps loaded before any is used
+    for (int i0 = first + threadIdx.x; i0 < end; i0 += kVerifyThreads * kFlight) {
+      float p[kFlight][N], q[kFlight][N], e[kFlight][N];
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        const int i = i0 + k * kVerifyThreads;
+        if (i >= end) break;
+        load_probs<kType, N>(a.target, row + static_cast<int64_t>(i) * N, p[k]);
+        load_probs<kProbF32, N>(noise, static_cast<int64_t>(i) * N, e[k]);
+        if (minus) load_probs<kType, N>(a.draft, drow + static_cast<int64_t>(i) * N, q[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        const int i = i0 + k * kVerifyThreads;
+        if (i >= end) break;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float w = minus ? p[k][j] - q[k][j] : p[k][j];
+          if (!(w > 0.0f && w >= bar * e[k][j])) continue;
+          const int v = i * N + j;
+          bool out = false;
+          if (residual && !minus)
+            for (int t = 0; t < tried; ++t) out = out || s_token[t] == v;
+          if (out) continue;
+          const float score = __fdiv_rn(w, e[k][j]);
+          if (score > best) {
+            best = score;
+            bar = best * 0.9999990f;
+            index = v;
+          }
         }
       }
-      if (!(w > 0.0f)) continue;
-      const float score = __fdiv_rn(w, a.noise[b * V + v]);
-      if (score > best) {
-        best = score;
-        index = v;
-      }
     }
+    unsigned long long key = best > 0.0f ? race_key(best, index) : 0ull;
+#pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
-      const float s = __shfl_xor_sync(0xffffffffu, best, off);
-      const int i = __shfl_xor_sync(0xffffffffu, index, off);
-      if (s > best || (s == best && i < index)) {
-        best = s;
-        index = i;
-      }
+      const unsigned long long o = __shfl_xor_sync(0xffffffffu, key, off);
+      key = o > key ? o : key;
     }
+    if (lane == 0) s_warp[warp] = key;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) {
-      s_score[threadIdx.x >> 5] = best;
-      s_index[threadIdx.x >> 5] = index;
-    }
-    __syncthreads();
-    best = 0.0f;
-    index = INT_MAX;
-    for (int i = 0; i < kVerifyThreads / 32; ++i)
-      if (s_score[i] > best || (s_score[i] == best && s_index[i] < index)) {
-        best = s_score[i];
-        index = s_index[i];
+    if (warp == 0) {
+      key = lane < kVerifyThreads / 32 ? s_warp[lane] : 0ull;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) {
+        const unsigned long long o = __shfl_xor_sync(0xffffffffu, key, off);
+        key = o > key ? o : key;
       }
-    if (index != INT_MAX || !residual) {
-      if (threadIdx.x == 0) {
-        const int next = index != INT_MAX ? index : 0;
-        if (a.tokens_64)
-          static_cast<long long*>(a.next)[b] = next;
-        else
-          static_cast<int*>(a.next)[b] = next;
-      }
-      return;
+      if (lane < ranks) store_remote(&s_best[attempt][rank], lane, key);
     }
+    cluster_sync();
+    key = 0ull;
+    for (unsigned r = 0; r < ranks; ++r) key = s_best[attempt][r] > key ? s_best[attempt][r] : key;
+    // Nothing left after the refusals: once more, from p itself.  (The same
+    // decision in every CTA: all see the same keys.)
+    if (key == 0ull && residual) continue;
+    if (rank == 0 && threadIdx.x == 0) {
+      const int next = key != 0ull ? static_cast<int>(0xffffffffu - static_cast<unsigned>(key)) : 0;
+      if (a.tokens_64)
+        static_cast<long long*>(a.next)[b] = next;
+      else
+        static_cast<int*>(a.next)[b] = next;
+    }
+    return;
   }
 }
 
-// One CTA per (sequence and layer, head): the accepted rows, 16 bytes a thread.
-__global__ void __launch_bounds__(128) commit_kernel(const CommitArgs a) {
-  const int64_t b = blockIdx.x % a.B, layer = blockIdx.x / a.B, h = blockIdx.y;
-  const bool is_v = blockIdx.z != 0;
+constexpr int kCommitThreads = 256;
+constexpr int kCommitHeads = 4;
+
+// CTA (b and layer, four heads): a thread has one 16-byte chunk of a row and
+// copies it for K and V of all its heads, eight loads in flight; the paths are
+// short, so it is bound by the latency of path, row and store.
+__global__ void __launch_bounds__(kCommitThreads) commit_kernel(const __grid_constant__ CommitArgs a, int chunks, int rows) {
+  const int64_t b = blockIdx.x % a.B, layer = blockIdx.x / a.B;
+  const int h0 = blockIdx.y * kCommitHeads, heads = min(kCommitHeads, static_cast<int>(a.H) - h0);
   const int n = min(max(a.path_lens[b], 0), static_cast<int>(a.T));
   const int start = min(max(a.kv_lens[b], 0), static_cast<int>(a.L));
   const int fit = min(n, static_cast<int>(a.L) - start);
-  if (blockIdx.y == 0 && layer == 0 && !is_v && threadIdx.x == 0) {
+  if (h0 == 0 && layer == 0 && threadIdx.x == 0) {
     a.new_lens[b] = start + fit;
     if (fit < n) atomicCAS(a.status, kOk, kErrTooLarge);
   }
-  const int64_t* cs = a.strides + (is_v ? 4 : 0);
-  const int64_t* ts = a.strides + (is_v ? 12 : 8);
-  uint16_t* dst = static_cast<uint16_t*>(is_v ? a.v : a.k) + layer * cs[0] + b * cs[1] + h * cs[2];
-  const uint16_t* src = static_cast<const uint16_t*>(is_v ? a.v_tree : a.k_tree) + layer * ts[0] + b * ts[1] + h * ts[2];
-  const int chunks = static_cast<int>(a.D / 8);
-  for (int u = threadIdx.x; u < fit * chunks; u += blockDim.x) {
-    const int i = u / chunks, c = u % chunks * 8;
+  const int lane_row = threadIdx.x / chunks, c = threadIdx.x % chunks * 8;
+  if (lane_row >= rows) return;
+  const int64_t* st = a.strides;  // k, v, k_tree, v_tree x (layer, batch, head, row)
+  uint16_t* k = static_cast<uint16_t*>(a.k) + layer * st[0] + b * st[1] + h0 * st[2] + c;
+  uint16_t* v = static_cast<uint16_t*>(a.v) + layer * st[4] + b * st[5] + h0 * st[6] + c;
+  const uint16_t* kt = static_cast<const uint16_t*>(a.k_tree) + layer * st[8] + b * st[9] + h0 * st[10] + c;
+  const uint16_t* vt = static_cast<const uint16_t*>(a.v_tree) + layer * st[12] + b * st[13] + h0 * st[14] + c;
+  for (int i = lane_row; i < fit; i += rows) {
     const int node = a.path[b * a.T + i];
     if (node < 0 || node >= a.T) {
       atomicCAS(a.status, kOk, kErrInvalidArgument);
       continue;
     }
-    *reinterpret_cast<uint4*>(dst + (start + i) * cs[3] + c) = *reinterpret_cast<const uint4*>(src + node * ts[3] + c);
+    uint4 x[kCommitHeads], y[kCommitHeads];
+#pragma unroll
+    for (int h = 0; h < kCommitHeads; ++h)
+      if (h < heads) {
+        x[h] = *reinterpret_cast<const uint4*>(kt + h * st[10] + node * st[11]);
+        y[h] = *reinterpret_cast<const uint4*>(vt + h * st[14] + node * st[15]);
+      }
+#pragma unroll
+    for (int h = 0; h < kCommitHeads; ++h)
+      if (h < heads) {
+        *reinterpret_cast<uint4*>(k + h * st[2] + (start + i) * st[3]) = x[h];
+        *reinterpret_cast<uint4*>(v + h * st[6] + (start + i) * st[7]) = y[h];
+      }
   }
+}
+
+template <int kType, int N>
+int launch_verify_t(const VerifyArgs& a, int cluster) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.B * cluster));
+  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.stream = a.stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, verify_kernel<kType, N>, a) != cudaSuccess) {
+    cudaGetLastError();
+    return kErrLaunch;
+  }
+  return kOk;
 }
 
 }  // namespace
 
 int launch_verify(const VerifyArgs& a) {
-  const unsigned grid = static_cast<unsigned>(a.B);
-  if (a.type == kProbF32)
-    verify_kernel<kProbF32><<<grid, kVerifyThreads, 0, a.stream>>>(a);
-  else if (a.type == kProbBf16)
-    verify_kernel<kProbBf16><<<grid, kVerifyThreads, 0, a.stream>>>(a);
-  else
-    verify_kernel<kProbF16><<<grid, kVerifyThreads, 0, a.stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+  // CTAs of a sequence: enough that the batch fills the device twice over, as
+  // long as each has a thread's worth of loads.
+  int cluster = 1;
+  while (cluster < kVerifyMaxCluster && a.B * cluster < 148 * 4 && a.V >= kVerifyThreads * 2 * cluster) cluster *= 2;
+  // Four entries a load where every row starts on their boundary.
+  const uintptr_t bytes = a.type == kProbF32 ? 16 : 8;
+  bool wide = a.V % 4 == 0 && a.target_stride[0] % 4 == 0 && a.target_stride[1] % 4 == 0 &&
+              reinterpret_cast<uintptr_t>(a.target) % bytes == 0 && reinterpret_cast<uintptr_t>(a.noise) % 16 == 0;
+  if (a.draft != nullptr)
+    wide = wide && a.draft_stride[0] % 4 == 0 && a.draft_stride[1] % 4 == 0 &&
+           reinterpret_cast<uintptr_t>(a.draft) % bytes == 0;
+  switch (a.type) {
+    case kProbF32: return wide ? launch_verify_t<kProbF32, 4>(a, cluster) : launch_verify_t<kProbF32, 1>(a, cluster);
+    case kProbBf16: return wide ? launch_verify_t<kProbBf16, 4>(a, cluster) : launch_verify_t<kProbBf16, 1>(a, cluster);
+    default: return wide ? launch_verify_t<kProbF16, 4>(a, cluster) : launch_verify_t<kProbF16, 1>(a, cluster);
+  }
 }
 
 int launch_commit(const CommitArgs& a) {
-  const dim3 grid(static_cast<unsigned>(a.layers * a.B), static_cast<unsigned>(a.H), 2);
-  commit_kernel<<<grid, 128, 0, a.stream>>>(a);
+  const int chunks = static_cast<int>(a.D / 8);
+  const dim3 grid(static_cast<unsigned>(a.layers * a.B), static_cast<unsigned>((a.H + kCommitHeads - 1) / kCommitHeads));
+  commit_kernel<<<grid, kCommitThreads, 0, a.stream>>>(a, chunks, kCommitThreads / chunks);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 

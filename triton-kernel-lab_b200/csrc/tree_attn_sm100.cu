@@ -49,23 +49,22 @@ namespace {
 template <int D, int kT, int kRep>
 struct TreeCfg {
   static_assert(kRep == 1 || kT == 1, "copies fill one tile");
-  static constexpr int kMinBlocks = (D == 64 && kRep == 1) ? 2 : 1;
-  // One tile per CTA and SM: a warpgroup of its own for the epilogue and two
-  // O buffers, so a segment's end does not hold up the next one's tiles, and a
-  // second S buffer, so S(j + 1) runs under the softmax of S(j).  Two CTAs or
-  // two tiles cover each other instead.
-  static constexpr bool kEpi = kT == 1 && kMinBlocks == 1;
+  // One tile per CTA: a warpgroup of its own for the epilogue and two O
+  // buffers, so a segment's end does not hold up the next one's tiles, and a
+  // second S buffer, so S(j + 1) runs under the softmax of S(j).  Two tiles
+  // cover each other instead (and fill tensor memory at D = 128).
+  static constexpr bool kEpi = kT == 1;
   static constexpr int kLook = kEpi ? 2 : 1;
   static constexpr int kThreads = 128 * (1 + kT + (kEpi ? 1 : 0));
   // Stages of K and of V.
-  static constexpr int kStages = (D == 64 && kRep > 1) ? 5 : 3;
-  static constexpr int kVStages = (D == 64 && kRep > 1) ? 4 : (kT == 1 && kRep == 1) ? 3 : 2;
-  static constexpr int kQBufs = (D == 64 && kRep > 1) ? 2 : 1;
+  static constexpr int kStages = (D == 64) ? 5 : 3;
+  static constexpr int kVStages = (D == 64) ? 4 : (kT == 1 && kRep == 1) ? 3 : 2;
+  static constexpr int kQBufs = (D == 64 && kT == 1) ? 2 : 1;
   static constexpr int kRows = kT * kTileRows / kRep;  // query rows per CTA
   // 0: launched with registers to spare, no redistribution.
-  static constexpr int kLaunchRegs = (kMinBlocks == 2) ? 128 : (kRep == 1) ? 168 : 0;
+  static constexpr int kLaunchRegs = (kRep == 1) ? 168 : 0;
   static constexpr int kRegsCtrl = 56;
-  static constexpr int kRegsWork = (kMinBlocks == 2) ? 200 : 224;  // of the other warpgroups
+  static constexpr int kRegsWork = 224;  // of the other warpgroups
   static_assert(kLaunchRegs == 0 || kRegsCtrl + (kThreads / 128 - 1) * kRegsWork <= kThreads / 128 * kLaunchRegs,
                 "register split exceeds the launch");
   static constexpr int kTileBytes = kTileRows * D * 2;
@@ -80,7 +79,7 @@ struct TreeCfg {
   static constexpr int kCtlOff = kBarOff + kNumBars * 8;
   static constexpr int kMlOff = (kCtlOff + 16 + 32 + 64 + 7) / 8 * 8;  // after control, first segment, scan
   static constexpr int kSmemBytes = kMlOff + (kEpi ? 2 * kTileRows * 8 : 0);  // m and l of a segment's rows, two buffers
-  static constexpr uint32_t kTmemCols = (kMinBlocks == 2) ? 256 : 512;
+  static constexpr uint32_t kTmemCols = 512;
   // O of query tile x, or O buffer x, at column x D; the S buffers from here.
   static constexpr uint32_t kColS0 = (kEpi ? 2 : kT) * D;
 };
@@ -410,7 +409,7 @@ __device__ __forceinline__ void finish_copies(bool ok, uint32_t o_addr, int r, b
 }
 
 template <int D, int kT, int kRep, bool kBf16>
-__global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, TreeCfg<D, kT, kRep>::kMinBlocks)
+__global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_kt,
                      const __grid_constant__ CUtensorMap tm_vt, const __grid_constant__ TreeShape shape,
@@ -965,18 +964,17 @@ struct TreeGrid {
   size_t plan_bytes, ml_bytes, o_bytes;
 };
 
-constexpr int tree_tiles_per_cta(int64_t D, int64_t R) { return D > 64 && R > kTileRows ? 2 : 1; }
+constexpr int tree_tiles_per_cta(int64_t R) { return R > kTileRows ? 2 : 1; }
 constexpr int tree_copies(int64_t R) { return R <= 32 ? 4 : R <= 64 ? 2 : 1; }
 
 TreeGrid tree_grid(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms) {
-  const int64_t group_rows = tree_tiles_per_cta(D, G * T) * kTileRows / tree_copies(G * T);
+  const int64_t group_rows = tree_tiles_per_cta(G * T) * kTileRows / tree_copies(G * T);
   const int64_t width = D > 64 ? 128 : 64;
-  const int64_t resident = sms * (width == 64 && tree_copies(G * T) == 1 ? 2 : 1);
   TreeGrid t;
   const int64_t groups = (G * T + group_rows - 1) / group_rows;
   const int64_t tiles = B * Hkv * ((L + kTileRows - 1) / kTileRows + (T + kTileRows - 1) / kTileRows + kItemCost);
   t.groups = static_cast<int>(groups);
-  t.runs = static_cast<int>(std::max<int64_t>(1, std::min(resident / groups, tiles)));
+  t.runs = static_cast<int>(std::max<int64_t>(1, std::min(sms / groups, tiles)));
   const size_t rows = static_cast<size_t>(groups) * t.runs * 2 * group_rows;
   t.cuts = static_cast<int>(std::min<int64_t>(B * Hkv, t.runs));
   t.plan_bytes = (static_cast<size_t>(t.cuts) * sizeof(int4) + 255) / 256 * 256;
@@ -1009,7 +1007,7 @@ int launch_tree_combine(const TreeAttnArgs& a, const TreeGrid& t, const TreeShap
 template <int D, int kT, int kRep, bool kBf16>
 int launch_tree_t(const TreeAttnArgs& a, const TreeGrid& t) {
   using C = TreeCfg<D, kT, kRep>;
-  static_assert(C::kSmemBytes + 1024 <= 233472 / C::kMinBlocks, "shared memory exceeds the SM's");
+  static_assert(C::kSmemBytes <= 232448, "shared memory exceeds the sm_100 limit");
   auto kern = tree_attn_kernel<D, kT, kRep, kBf16>;
   if (int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::kSmemBytes, C::kLaunchRegs, nullptr)) return rc;
   const TreeShape shape{a.kv_lens, a.tree_sizes, a.parents, a.parent_stride, static_cast<int>(a.B),
@@ -1040,9 +1038,7 @@ int launch_tree_r(const TreeAttnArgs& a, const TreeGrid& t) {
     case 2: return launch_tree_t<D, 1, 2, kBf16>(a, t);
     default: break;
   }
-  if constexpr (D == 128) {
-    if (tree_tiles_per_cta(a.D, a.G * a.T) == 2) return launch_tree_t<128, 2, 1, kBf16>(a, t);
-  }
+  if (tree_tiles_per_cta(a.G * a.T) == 2) return launch_tree_t<D, 2, 1, kBf16>(a, t);
   return launch_tree_t<D, 1, 1, kBf16>(a, t);
 }
 
