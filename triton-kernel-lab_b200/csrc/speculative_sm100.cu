@@ -17,8 +17,8 @@
 // or p_n where n has no child; p_n also where the residual has no mass left.
 // The emitted tokens are then distributed as the target's own samples.
 //
-// Whether child c passes depends on its siblings alone, so every node is
-// tested at once and the walk only follows the chosen children.
+// Every node's probability is loaded at once; the walk itself is a warp's, over
+// the visited nodes only.
 #include "attn_launch.h"
 #include "sm100_primitives.cuh"
 
@@ -72,6 +72,7 @@ __device__ __forceinline__ void store_remote(const void* mine, unsigned rank, un
 
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyMaxCluster = 8;
+constexpr int kFilterWords = 256;
 
 // N consecutive probabilities (or noise values), fp32; vector loads at N = 4.
 template <int kType, int N>
@@ -105,16 +106,21 @@ __device__ __forceinline__ void load_probs(const void* p, int64_t i, float (&f)[
 // probabilities, the row) where there are few: the noise, which depends on
 // none, is brought into L2 meanwhile.
 //
-// The race divides only where it may win: w / e rounds to more than `best`
-// only if w > best e (1 - 2^-23), tested with a margin, so nearly every
-// element costs a multiplication and a comparison.
-template <int kType, int N>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_constant__ VerifyArgs a) {
-  __shared__ int s_parent[kTreeMaxNodes], s_child[kTreeMaxNodes], s_path[kTreeMaxNodes];
-  __shared__ long long s_token[kTreeMaxNodes];
-  __shared__ float s_prob[kTreeMaxNodes], s_left[kTreeMaxNodes];
-  __shared__ unsigned char s_pass[kTreeMaxNodes];
-  __shared__ int s_last, s_length, s_tried;
+// The race is run on w times the hardware reciprocal of e (a few operations an
+// element, no branch); a thread then divides for its own best only, or, if its
+// second is within 2^-19 of it (16-bit probabilities and small variates take few
+// values, so that happens), its warp for all its elements: the result is that
+// of the rounded quotients.  Dividing wherever a
+// thread's or a warp's best so far might be beaten bound it: B = 32, 128000
+// entries, bf16, 24 to 45 us.
+template <int kType, int N, bool kDraft>
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_constant__ VerifyArgs a) {
+  __shared__ int s_parent[kTreeMaxNodes], s_path[kTreeMaxNodes];
+  __shared__ long long s_token[kTreeMaxNodes], s_list[kTreeMaxNodes];
+  __shared__ float s_prob[kTreeMaxNodes], s_uniform[kTreeMaxNodes];
+  __shared__ bool s_pass[kTreeMaxNodes];
+  __shared__ int s_length, s_tried;
+  __shared__ unsigned s_filter[kFilterWords];
   __shared__ unsigned long long s_warp[kVerifyThreads / 32], s_best[2][kVerifyMaxCluster];
   cluster_arrive();  // waited for before the first store to another CTA's shared memory
   const unsigned rank = cluster_rank(), ranks = cluster_size();
@@ -136,63 +142,80 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     const long long x = token_at(a, b * T + c);
     const bool real = n >= 0 && x >= 0 && x < V;
     const float p = real ? prob_at<kType>(a.target, b * a.target_stride[0] + n * a.target_stride[1] + x) : 0.0f;
+    const float u = a.uniforms[b * T + c];
     bool pass = false;
-    if (a.draft != nullptr && p > 0.0f)
-      pass = a.uniforms[b * T + c] * prob_at<kType>(a.draft, b * a.draft_stride[0] + n * a.draft_stride[1] + x) < p;
+    if (kDraft && p > 0.0f)
+      pass = u * prob_at<kType>(a.draft, b * a.draft_stride[0] + n * a.draft_stride[1] + x) < p;
     s_parent[c] = n;
     s_token[c] = x;
     s_prob[c] = p;
+    s_uniform[c] = u;
     s_pass[c] = pass;
-    s_child[c] = -1;
   }
-  if (threadIdx.x == 0) s_tried = 0;
+  for (int i = threadIdx.x; i < kFilterWords; i += kVerifyThreads) s_filter[i] = 0;
   __syncthreads();
-  if (a.draft == nullptr) {
-    // A warp per node.  Its token's mass, unless an earlier sibling tried it ...
-    for (int c = warp; c < size; c += kVerifyThreads / 32) {
-      const int n = s_parent[c];
-      bool again = false;
-      if (n >= 0)
-        for (int s = n + 1 + lane; s < c; s += 32) again = again || (s_parent[s] == n && s_token[s] == s_token[c]);
-      again = __any_sync(0xffffffffu, again);
-      if (lane == 0) s_left[c] = again || !(s_prob[c] > 0.0f) ? 0.0f : s_prob[c];
-    }
-    __syncthreads();
-    // ... against what its earlier siblings left.
-    for (int c = warp; c < size; c += kVerifyThreads / 32) {
-      const int n = s_parent[c];
-      float mass = 0.0f;
-      if (n >= 0)
-        for (int s = n + 1 + lane; s < c; s += 32) mass += s_parent[s] == n ? s_left[s] : 0.0f;
+  if (warp == 0) {
+    // The walk: at each node its children in order, 32 candidates at a time.
+    int length = 0, tried = 0;
+    for (int n = size > 0 ? 0 : -1; n >= 0;) {
+      if (lane == 0) s_path[length] = n;
+      ++length;
+      tried = 0;
+      int next = -1;
+      float mass = 0.0f;  // of the children refused so far
+      for (int c0 = (n + 1) & ~31; c0 < size; c0 += 32) {
+        const int c = c0 + lane;
+        const bool child = c > n && c < size && s_parent[c] == n;
+        const unsigned all = __ballot_sync(0xffffffffu, child), before = all & ((1u << lane) - 1u);
+        if (all == 0) continue;
+        const long long x = child ? s_token[c] : -1;
+        bool pass;
+        if constexpr (kDraft) {
+          pass = child && s_pass[c];
+        } else {
+          bool again = (__match_any_sync(0xffffffffu, x) & before) != 0;
+          for (int t = 0; t < tried; ++t) again = again || s_list[t] == x;
+          const float left = child && !again && s_prob[c] > 0.0f ? s_prob[c] : 0.0f;
+          float upto = left;
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, off);
-      if (lane == 0 && n >= 0)
-        s_pass[c] = s_left[c] > 0.0f && a.uniforms[b * T + c] * fmaxf(1.0f - mass, 0.0f) < s_left[c];
+          for (int off = 1; off < 32; off <<= 1) {
+            const float o = __shfl_up_sync(0xffffffffu, upto, off);
+            if (lane >= off) upto += o;
+          }
+          const float earlier = __shfl_up_sync(0xffffffffu, upto, 1);
+          pass = left > 0.0f && s_uniform[c] * fmaxf(1.0f - (mass + (lane > 0 ? earlier : 0.0f)), 0.0f) < left;
+          mass += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        const unsigned passed = __ballot_sync(0xffffffffu, pass);
+        if (passed != 0) {
+          next = c0 + __ffs(passed) - 1;
+          break;
+        }
+        if (child) s_list[tried + __popc(before)] = x;
+        tried += __popc(all);
+        __syncwarp();
+      }
+      n = next;
     }
-    __syncthreads();
-  }
-  for (int c = threadIdx.x; c < size; c += kVerifyThreads)
-    if (s_pass[c]) {
-      const int n = s_parent[c];
-      bool lead = true;
-      for (int s = n + 1; s < c; ++s) lead = lead && !(s_parent[s] == n && s_pass[s]);
-      if (lead) s_child[n] = c;
+    // A filter over the steps that hold a tried token.
+    for (int t = lane; !kDraft && t < tried; t += 32)
+      if (s_list[t] >= 0 && s_list[t] < V) {
+        const unsigned i = static_cast<unsigned>(s_list[t]) / N;
+        atomicOr(&s_filter[(i >> 5) % kFilterWords], 1u << (i & 31));
+      }
+    if (lane == 0) {
+      s_length = length;
+      s_tried = tried;
     }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int length = 0;
-    for (int n = size > 0 ? 0 : -1; n >= 0; n = s_child[n]) s_path[length++] = n;
-    s_length = length;
-    s_last = length > 0 ? s_path[length - 1] : -1;
   }
   __syncthreads();
   cluster_wait();
-  const int last = s_last, length = s_length;
+  const int length = s_length, tried = s_tried;
   if (rank == 0) {
     for (int i = threadIdx.x; i < T; i += kVerifyThreads) a.path[b * T + i] = i < length ? s_path[i] : -1;
     if (threadIdx.x == 0) a.path_lens[b] = length;
   }
-  if (last < 0) {  // the same in every CTA of the cluster
+  if (length == 0) {  // the same in every CTA of the cluster
     if (rank == 0 && threadIdx.x == 0) {
       if (a.tokens_64)
         static_cast<long long*>(a.next)[b] = -1;
@@ -201,64 +224,72 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     }
     return;
   }
-  // The tokens tried at the last node (s_token's first entries from here on).
-  __syncthreads();
-  if (warp == 0) {
-    int tried = 0;
-    for (int c0 = last + 1; c0 < size; c0 += 32) {
-      const int c = c0 + lane;
-      const bool mine = c < size && s_parent[c] == last;
-      const long long x = mine ? s_token[c] : 0;
-      const unsigned all = __ballot_sync(0xffffffffu, mine);
-      if (mine) s_token[tried + __popc(all & ((1u << lane) - 1u))] = x;
-      tried += __popc(all);
-      __syncwarp();
-    }
-    if (lane == 0) s_tried = tried;
-  }
-  __syncthreads();
-  const int tried = s_tried;
+  const int last = s_path[length - 1];
   const int64_t row = b * a.target_stride[0] + last * a.target_stride[1];
-  const int64_t drow = a.draft != nullptr ? b * a.draft_stride[0] + last * a.draft_stride[1] : 0;
+  const int64_t drow = kDraft ? b * a.draft_stride[0] + last * a.draft_stride[1] : 0;
   for (int attempt = 0; attempt < 2; ++attempt) {
     const bool residual = attempt == 0 && tried > 0;
-    const bool minus = residual && a.draft != nullptr;
-    float best = 0.0f, bar = 0.0f;
-    int index = 0;
-    constexpr int kFlight = 16 / N / (N > 1 ? 2 : 1);  // steps loaded before any is used
+    const bool minus = kDraft && residual;
+    const bool skips = !kDraft && residual;
+    auto was_tried = [&](int v) {
+      bool out = false;
+      for (int t = 0; t < tried; ++t) out = out || s_list[t] == v;
+      return out;
+    };
+    float best = 0.0f, second = 0.0f;
+    int index = -1;
+    constexpr int kFlight = N > 1 ? (kDraft ? 2 : 4) : 8;  // steps loaded before any is used
     for (int i0 = first + threadIdx.x; i0 < end; i0 += kVerifyThreads * kFlight) {
       float p[kFlight][N], q[kFlight][N], e[kFlight][N];
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
         const int i = i0 + k * kVerifyThreads;
-        if (i >= end) break;
-        load_probs<kType, N>(a.target, row + static_cast<int64_t>(i) * N, p[k]);
-        load_probs<kProbF32, N>(noise, static_cast<int64_t>(i) * N, e[k]);
-        if (minus) load_probs<kType, N>(a.draft, drow + static_cast<int64_t>(i) * N, q[k]);
+#pragma unroll
+        for (int j = 0; j < N; ++j) p[k][j] = q[k][j] = 0.0f, e[k][j] = 1.0f;
+        if (i < end) {
+          load_probs<kType, N>(a.target, row + static_cast<int64_t>(i) * N, p[k]);
+          load_probs<kProbF32, N>(noise, static_cast<int64_t>(i) * N, e[k]);
+          if (minus) load_probs<kType, N>(a.draft, drow + static_cast<int64_t>(i) * N, q[k]);
+        }
       }
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
         const int i = i0 + k * kVerifyThreads;
-        if (i >= end) break;
+        if (skips && ((s_filter[(i >> 5) % kFilterWords] >> (i & 31)) & 1u)) {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if (was_tried(i * N + j)) p[k][j] = 0.0f;
+        }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const float w = minus ? p[k][j] - q[k][j] : p[k][j];
-          if (!(w > 0.0f && w >= bar * e[k][j])) continue;
-          const int v = i * N + j;
-          bool out = false;
-          if (residual && !minus)
-            for (int t = 0; t < tried; ++t) out = out || s_token[t] == v;
-          if (out) continue;
-          const float score = __fdiv_rn(w, e[k][j]);
-          if (score > best) {
-            best = score;
-            bar = best * 0.9999990f;
-            index = v;
-          }
+          float r;
+          asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e[k][j]));
+          const float score = (kDraft ? p[k][j] - q[k][j] : p[k][j]) * r;
+          const bool wins = score > best;
+          second = fmaxf(second, wins ? best : score);
+          best = wins ? score : best;
+          index = wins ? i * N + j : index;
         }
       }
     }
-    unsigned long long key = best > 0.0f ? race_key(best, index) : 0ull;
+    // The thread's exact best; where its second is too near, the warp divides
+    // for all of its elements.
+    auto exact = [&](int v) {
+      float w = prob_at<kType>(a.target, row + v);
+      if (minus) w -= prob_at<kType>(a.draft, drow + v);
+      const float score = __fdiv_rn(w, noise[v]);
+      return score > 0.0f && !(skips && was_tried(v)) ? race_key(score, v) : 0ull;
+    };
+    const bool clear = index < 0 || (second < best * 0.999998f && best < INFINITY);
+    unsigned long long key = clear && index >= 0 ? exact(index) : 0ull;
+    for (unsigned close = __ballot_sync(0xffffffffu, !clear); close != 0; close &= close - 1) {
+      for (int i = first + warp * 32 + __ffs(close) - 1 + lane * kVerifyThreads; i < end; i += 32 * kVerifyThreads)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const unsigned long long mine = exact(i * N + j);
+          key = mine > key ? mine : key;
+        }
+    }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
       const unsigned long long o = __shfl_xor_sync(0xffffffffu, key, off);
@@ -337,7 +368,7 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const __grid_con
   }
 }
 
-template <int kType, int N>
+template <int kType, int N, bool kDraft>
 int launch_verify_t(const VerifyArgs& a, int cluster) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.B * cluster));
@@ -350,20 +381,27 @@ int launch_verify_t(const VerifyArgs& a, int cluster) {
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, verify_kernel<kType, N>, a) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, verify_kernel<kType, N, kDraft>, a) != cudaSuccess) {
     cudaGetLastError();
     return kErrLaunch;
   }
   return kOk;
 }
 
+template <int kType>
+int launch_verify_n(const VerifyArgs& a, int cluster, bool wide) {
+  if (a.draft != nullptr)
+    return wide ? launch_verify_t<kType, 4, true>(a, cluster) : launch_verify_t<kType, 1, true>(a, cluster);
+  return wide ? launch_verify_t<kType, 4, false>(a, cluster) : launch_verify_t<kType, 1, false>(a, cluster);
+}
+
 }  // namespace
 
 int launch_verify(const VerifyArgs& a) {
-  // CTAs of a sequence: enough that the batch fills the device twice over, as
-  // long as each has a thread's worth of loads.
+  // CTAs of a sequence: one an SM (each walks the tree again), as long as each
+  // has a thread's worth of loads.
   int cluster = 1;
-  while (cluster < kVerifyMaxCluster && a.B * cluster < 148 * 4 && a.V >= kVerifyThreads * 2 * cluster) cluster *= 2;
+  while (cluster < kVerifyMaxCluster && a.B * cluster < 148 && a.V >= kVerifyThreads * 2 * cluster) cluster *= 2;
   // Four entries a load where every row starts on their boundary.
   const uintptr_t bytes = a.type == kProbF32 ? 16 : 8;
   bool wide = a.V % 4 == 0 && a.target_stride[0] % 4 == 0 && a.target_stride[1] % 4 == 0 &&
@@ -372,9 +410,9 @@ int launch_verify(const VerifyArgs& a) {
     wide = wide && a.draft_stride[0] % 4 == 0 && a.draft_stride[1] % 4 == 0 &&
            reinterpret_cast<uintptr_t>(a.draft) % bytes == 0;
   switch (a.type) {
-    case kProbF32: return wide ? launch_verify_t<kProbF32, 4>(a, cluster) : launch_verify_t<kProbF32, 1>(a, cluster);
-    case kProbBf16: return wide ? launch_verify_t<kProbBf16, 4>(a, cluster) : launch_verify_t<kProbBf16, 1>(a, cluster);
-    default: return wide ? launch_verify_t<kProbF16, 4>(a, cluster) : launch_verify_t<kProbF16, 1>(a, cluster);
+    case kProbF32: return launch_verify_n<kProbF32>(a, cluster, wide);
+    case kProbBf16: return launch_verify_n<kProbBf16>(a, cluster, wide);
+    default: return launch_verify_n<kProbF16>(a, cluster, wide);
   }
 }
 
