@@ -25,8 +25,6 @@ contexts.  The tables are constants: no gradient flows to them.
 
 from __future__ import annotations
 
-import ctypes
-import functools
 import math
 from typing import Any
 
@@ -34,7 +32,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from tklab import _native
-from tklab.kernels.flash_attention import _NATIVE_DTYPE, _after_launch, _on_device, _stream
+from tklab.kernels._plans import Plans, _after_launch, _stream, at_device, dense, meta, row_strides, stride_array
+from tklab.kernels.flash_attention import _NATIVE_DTYPE
 
 ROTARY_LAYOUTS = ("half", "interleaved")
 ROTARY_SCALINGS = ("none", "linear", "ntk", "yarn", "bands")
@@ -106,35 +105,22 @@ def rotary_tables(
     return (gain * angles.cos()).to(torch.float32), (gain * angles.sin()).to(torch.float32)
 
 
-@functools.lru_cache(maxsize=1024)
-def _strides3(batch: int, head: int, row: int) -> ctypes.Array:
-    """The three strides as the C array that the library reads (never written)."""
-    return (ctypes.c_int64 * 3)(batch, head, row)
+_PLANS = Plans()
 
 
-def _rows(x: torch.Tensor) -> tuple[torch.Tensor, ctypes.Array]:
-    """``x`` (copied only if its rows cannot be read in place) and its (batch, head, row) strides."""
-    sb, sh, ss, sd = x.stride()
-    if sd != 1 or (sb | sh | ss) & 7 or x.data_ptr() & 15:
-        x = x.contiguous()
-        sb, sh, ss, _ = x.stride()
-        # contiguous() keeps odd strides of dimensions of size 1; they are never used.
-        sb, sh, ss = sb & ~7, sh & ~7, ss & ~7
-        if x.data_ptr() & 15 or x.stride(3) != 1:
-            x = x.clone(memory_format=torch.contiguous_format)
-    return x, _strides3(sb, sh, ss)
-
-
-def _validate(
+def _plan(
     q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
     positions: torch.Tensor | None, layout: str,
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
-    """Check the contract; return the tables as contiguous fp32 and the positions as (batch, seq)."""
+) -> tuple:
+    """Check the contract; return what a call with this metadata passes to the library.
+
+    The first entry says whether every tensor can be read in place.
+    """
     if layout not in ROTARY_LAYOUTS:
         raise ValueError(f"rotary layout must be one of {ROTARY_LAYOUTS}")
     if q.ndim != 4:
         raise ValueError("rotary expects q shaped (batch, heads, sequence, dim)")
-    batch, _, seq, head_dim = q.shape
+    batch, q_heads, seq, head_dim = q.shape
     if k is not None and (k.ndim != 4 or k.shape[0] != batch or k.shape[2] != seq or k.shape[3] != head_dim):
         raise ValueError("q and k must agree on batch, sequence and head_dim")
     if 0 in q.shape or (k is not None and 0 in k.shape):
@@ -160,43 +146,59 @@ def _validate(
     else:
         if positions.dtype not in (torch.int32, torch.int64) or positions.device != device:
             raise ValueError("positions must be an int32 or int64 tensor on q's device")
-        if positions.ndim == 1 and positions.shape[0] == seq:
-            positions = positions.expand(batch, seq)
-        if positions.shape != (batch, seq):
+        if positions.shape not in ((batch, seq), (seq,)):
             raise ValueError("positions must be shaped (batch, sequence) or (sequence,)")
-        positions = positions.contiguous()
-    if cos.dtype != torch.float32 or not cos.is_contiguous() or cos.data_ptr() & 15:
-        cos = cos.detach().to(torch.float32, copy=True, memory_format=torch.contiguous_format)
-    if sin.dtype != torch.float32 or not sin.is_contiguous() or sin.data_ptr() & 15:
-        sin = sin.detach().to(torch.float32, copy=True, memory_format=torch.contiguous_format)
-    return cos, sin, positions
+    q_strides = row_strides(q)
+    k_strides = (0, 0, 0) if k is None else row_strides(k)
+    in_place = (
+        q_strides is not None and k_strides is not None
+        and all(t.dtype == torch.float32 and t.is_contiguous() for t in (cos, sin))
+        and (positions is None or (positions.ndim == 2 and positions.is_contiguous()))
+    )
+    return (
+        in_place, q.get_device(), (batch, 0 if k is None else k.shape[1], seq, head_dim),
+        stride_array(*(q_strides or ())), stride_array(*(k_strides or ())),
+        0 if positions is None else int(positions.dtype == torch.int64),
+        batch, q_heads, 0 if k is None else k.shape[1], seq, head_dim, 2 * cos.shape[1], cos.shape[0],
+        _NATIVE_DTYPE[q.dtype], int(layout == "interleaved"),
+    )
+
+
+def _table(t: torch.Tensor) -> torch.Tensor:
+    t = t.detach()
+    return t.to(torch.float32, copy=bool(t.data_ptr() & 15), memory_format=torch.contiguous_format).contiguous()
 
 
 def _launch(
     q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
-    positions: torch.Tensor | None, layout: str, transpose: bool,
+    positions: torch.Tensor | None, layout: str, transpose: int,
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """The library call for validated arguments, into fresh contiguous outputs."""
-    batch, q_heads, seq, head_dim = q.shape
-    kv_heads = 0 if k is None else k.shape[1]
-    device = q.device
-    q, q_strides = _rows(q)
-    q_out = torch.empty((batch, q_heads, seq, head_dim), dtype=q.dtype, device=device)
-    k_out, k_strides = None, None
-    if k is not None:
-        k, k_strides = _rows(k)
-        k_out = torch.empty((batch, kv_heads, seq, head_dim), dtype=q.dtype, device=device)
-    with _on_device(device):
+    """Check (or recall) and make the library call, into fresh contiguous outputs."""
+    key = (
+        q.shape, q.stride(), q.dtype, q.get_device(), meta(k), cos.shape, cos.stride(), cos.dtype, cos.get_device(),
+        sin.shape, sin.stride(), sin.dtype, sin.get_device(), meta(positions), layout,
+    )
+    plan = _PLANS.get(key) or _PLANS.keep(key, _plan(q, k, cos, sin, positions, layout))
+    (in_place, device, k_shape, q_strides, k_strides, wide, batch, q_heads, kv_heads, seq, head_dim, rotary_dim, rows,
+     dtype, interleaved) = plan
+    q_ptr, k_ptr = q.data_ptr(), 0 if k is None else k.data_ptr()
+    cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
+    if not in_place or (q_ptr | k_ptr | cos_ptr | sin_ptr) & 15:
+        if positions is not None:
+            positions = positions.expand(batch, seq).contiguous()
+        return _launch(
+            dense(q), None if k is None else dense(k), _table(cos), _table(sin), positions, layout, transpose
+        )
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+    with at_device(device):
         status = _native.load().tk_rotary(
-            q.data_ptr(), None if k is None else k.data_ptr(), q_out.data_ptr(),
-            None if k_out is None else k_out.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-            None if positions is None else positions.data_ptr(),
-            0 if positions is None else int(positions.dtype == torch.int64),
-            batch, q_heads, kv_heads, seq, head_dim, 2 * cos.shape[1], cos.shape[0], q_strides, k_strides,
-            _NATIVE_DTYPE[q.dtype], int(layout == "interleaved"), int(transpose), _stream(q),
+            q_ptr, k_ptr, q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), cos_ptr, sin_ptr,
+            0 if positions is None else positions.data_ptr(), wide, batch, q_heads, kv_heads, seq, head_dim,
+            rotary_dim, rows, q_strides, k_strides, dtype, interleaved, transpose, _stream(q),
         )
     _native.check(status, "tk_rotary")
-    _after_launch(device)
+    _after_launch(q.device)
     return q_out, k_out
 
 
@@ -209,7 +211,7 @@ class _RotaryFunction(torch.autograd.Function):
         ctx.save_for_backward(cos, sin, positions)
         ctx.layout = layout
         ctx.set_materialize_grads(False)
-        return _launch(q, k, cos, sin, positions, layout, False)
+        return _launch(q, k, cos, sin, positions, layout, 0)
 
     @staticmethod
     @once_differentiable
@@ -218,9 +220,9 @@ class _RotaryFunction(torch.autograd.Function):
         cos, sin, positions = ctx.saved_tensors
         gq = gk = None
         if dq is not None:
-            gq, gk = _launch(dq, dk, cos, sin, positions, ctx.layout, True)
+            gq, gk = _launch(dq, dk, cos, sin, positions, ctx.layout, 1)
         elif dk is not None:
-            gk, _ = _launch(dk, None, cos, sin, positions, ctx.layout, True)
+            gk, _ = _launch(dk, None, cos, sin, positions, ctx.layout, 1)
         return gq, gk, None, None, None, None
 
 
@@ -241,7 +243,6 @@ def rotary(
     contiguous (batch, heads, seq, head_dim) tensors; differentiable in ``q``
     and ``k``.
     """
-    cos, sin, positions = _validate(q, k, cos, sin, positions, layout)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryFunction.apply(q, k, cos, sin, positions, layout)
-    return _launch(q, k, cos, sin, positions, layout, False)
+    return _launch(q, k, cos, sin, positions, layout, 0)
