@@ -241,3 +241,21 @@ def test_agrees_with_torch_rope_and_other_streams() -> None:
     side.synchronize()
     assert_rotated(y.cpu(), q.cpu(), torch_rope(q.double(), cos.double(), sin.double()).cpu())
     check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+def test_gradient_of_the_gradient_and_without_positions() -> None:
+    """The rotation is linear: its second derivative is the rotation of the cotangent's cotangent."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    cos, sin = rotary_tables(5, 64, device="cuda")
+    q = make((1, 2, 5, 64), torch.float16, gen).requires_grad_(True)
+    k = make((1, 1, 5, 64), torch.float16, gen).requires_grad_(True)
+    dq, dk = (make(x.shape, torch.float16, gen).requires_grad_(True) for x in (q, k))
+    gq, gk = torch.autograd.grad(rotary(q, k, cos, sin), (q, k), (dq, dk), create_graph=True)
+    v, w = make(q.shape, torch.float16, gen), make(k.shape, torch.float16, gen)
+    for got, x in zip(torch.autograd.grad((gq, gk), (dq, dk), (v, w)), (v, w), strict=True):
+        assert_rotated(got.cpu(), x.cpu(), rotary_reference(x.cpu(), cos.cpu(), sin.cpu()))
+    (g,) = torch.autograd.grad(rotary(q, k.detach(), cos, sin)[0], q, dq.detach())
+    assert torch.equal(g, gq)
+    check_device_status()

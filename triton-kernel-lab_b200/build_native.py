@@ -5,9 +5,12 @@ The library is compiled in-tree with nvcc for ``sm_100a`` only and placed at
 it travels with the source tree.  A second, test-only library,
 ``tklab/_lib/libtklab_selftest.so`` (``csrc/selftest/``: probes of the
 tcgen05 operand forms and of the FMA-pipe exponential), is built beside it;
-only the tests load it.  Run ``python build_native.py`` or call
-:func:`build`.  Each library is rebuilt only when one of its sources or
-headers is newer than it, unless ``force`` is set.
+only the tests load it.  ``tklab/_lib/_tklab_tensors.so``
+(``csrc/binding/``) is a Python extension that calls the library's serving
+entries on torch tensors; it is compiled against the installed torch.  Run
+``python build_native.py`` or call :func:`build`.  Each library is rebuilt
+only when one of its sources or headers is newer than it, unless ``force`` is
+set.
 """
 
 from __future__ import annotations
@@ -27,6 +30,8 @@ LIB_DIR = ROOT / "tklab" / "_lib"
 LIB_PATH = LIB_DIR / "libtklab_attn.so"
 SELFTEST_DIR = CSRC / "selftest"
 SELFTEST_LIB_PATH = LIB_DIR / "libtklab_selftest.so"
+BINDING_SOURCE = CSRC / "binding" / "tensors.cpp"
+BINDING_PATH = LIB_DIR / "_tklab_tensors.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CXX_FLAGS = [
@@ -106,10 +111,42 @@ def _build_one(src_dir: Path, lib_path: Path, obj_dir: Path, force: bool, verbos
     return lib_path
 
 
+def _build_binding(force: bool, verbose: bool) -> None:
+    """The Python extension, linked to the attention library beside it and to torch's libraries."""
+    import sysconfig
+
+    import torch
+
+    deps = [BINDING_SOURCE, INCLUDE / "tklab_attn.h"]
+    if not force and BINDING_PATH.exists() and all(d.stat().st_mtime <= BINDING_PATH.stat().st_mtime for d in deps):
+        return
+    gxx = shutil.which("g++")
+    if gxx is None:
+        raise RuntimeError("g++ not found: put it on PATH")
+    torch_dir = Path(torch.__file__).resolve().parent
+    cuda_dir = Path(_nvcc()).resolve().parent.parent
+    includes = [
+        torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include", cuda_dir / "include",
+        Path(sysconfig.get_paths()["include"]),
+    ]
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = [
+        gxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        *[arg for path in includes for arg in ("-isystem", str(path))],
+        str(BINDING_SOURCE), "-o", str(tmp),
+        "-L", str(LIB_DIR), "-l:" + LIB_PATH.name, "-Wl,-rpath,$ORIGIN",
+        "-L", str(torch_dir / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+    ]
+    _run(cmd, verbose)
+    os.replace(tmp, BINDING_PATH)
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
-    """Compile and link the attention library and the test-only library; return the former's path."""
+    """Compile and link the attention library, the test-only library and the tensor binding; return the first's path."""
     _build_one(CSRC, LIB_PATH, BUILD_DIR, force, verbose, ptxas_info)
     _build_one(SELFTEST_DIR, SELFTEST_LIB_PATH, BUILD_DIR / "selftest", force, verbose, ptxas_info)
+    _build_binding(force, verbose)
     return LIB_PATH
 
 

@@ -26,14 +26,11 @@ contexts.  The tables are constants: no gradient flows to them.
 from __future__ import annotations
 
 import math
-from typing import Any
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from tklab import _native
-from tklab.kernels._plans import Plans, _after_launch, _stream, at_device, dense, meta, row_strides, stride_array
-from tklab.kernels.flash_attention import _NATIVE_DTYPE
+from tklab._tensors import binding, dense
+from tklab.kernels.flash_attention import _NATIVE_DTYPE, _after_launch
 
 ROTARY_LAYOUTS = ("half", "interleaved")
 ROTARY_SCALINGS = ("none", "linear", "ntk", "yarn", "bands")
@@ -105,22 +102,13 @@ def rotary_tables(
     return (gain * angles.cos()).to(torch.float32), (gain * angles.sin()).to(torch.float32)
 
 
-_PLANS = Plans()
-
-
-def _plan(
-    q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
-    positions: torch.Tensor | None, layout: str,
+def _prepare(
+    q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None
 ) -> tuple:
-    """Check the contract; return what a call with this metadata passes to the library.
-
-    The first entry says whether every tensor can be read in place.
-    """
-    if layout not in ROTARY_LAYOUTS:
-        raise ValueError(f"rotary layout must be one of {ROTARY_LAYOUTS}")
+    """Check the contract; return the arguments with whatever the kernel cannot read in place copied."""
     if q.ndim != 4:
         raise ValueError("rotary expects q shaped (batch, heads, sequence, dim)")
-    batch, q_heads, seq, head_dim = q.shape
+    batch, _, seq, head_dim = q.shape
     if k is not None and (k.ndim != 4 or k.shape[0] != batch or k.shape[2] != seq or k.shape[3] != head_dim):
         raise ValueError("q and k must agree on batch, sequence and head_dim")
     if 0 in q.shape or (k is not None and 0 in k.shape):
@@ -148,82 +136,13 @@ def _plan(
             raise ValueError("positions must be an int32 or int64 tensor on q's device")
         if positions.shape not in ((batch, seq), (seq,)):
             raise ValueError("positions must be shaped (batch, sequence) or (sequence,)")
-    q_strides = row_strides(q)
-    k_strides = (0, 0, 0) if k is None else row_strides(k)
-    in_place = (
-        q_strides is not None and k_strides is not None
-        and all(t.dtype == torch.float32 and t.is_contiguous() for t in (cos, sin))
-        and (positions is None or (positions.ndim == 2 and positions.is_contiguous()))
-    )
-    return (
-        in_place, q.get_device(), (batch, 0 if k is None else k.shape[1], seq, head_dim),
-        stride_array(*(q_strides or ())), stride_array(*(k_strides or ())),
-        0 if positions is None else int(positions.dtype == torch.int64),
-        batch, q_heads, 0 if k is None else k.shape[1], seq, head_dim, 2 * cos.shape[1], cos.shape[0],
-        _NATIVE_DTYPE[q.dtype], int(layout == "interleaved"),
-    )
+        positions = positions.expand(batch, seq).contiguous()
 
+    def table(t: torch.Tensor) -> torch.Tensor:
+        t = t.detach().to(torch.float32).contiguous()
+        return t.clone() if t.data_ptr() % 16 else t
 
-def _table(t: torch.Tensor) -> torch.Tensor:
-    t = t.detach()
-    return t.to(torch.float32, copy=bool(t.data_ptr() & 15), memory_format=torch.contiguous_format).contiguous()
-
-
-def _launch(
-    q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
-    positions: torch.Tensor | None, layout: str, transpose: int,
-) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """Check (or recall) and make the library call, into fresh contiguous outputs."""
-    key = (
-        q.shape, q.stride(), q.dtype, q.get_device(), meta(k), cos.shape, cos.stride(), cos.dtype, cos.get_device(),
-        sin.shape, sin.stride(), sin.dtype, sin.get_device(), meta(positions), layout,
-    )
-    plan = _PLANS.get(key) or _PLANS.keep(key, _plan(q, k, cos, sin, positions, layout))
-    (in_place, device, k_shape, q_strides, k_strides, wide, batch, q_heads, kv_heads, seq, head_dim, rotary_dim, rows,
-     dtype, interleaved) = plan
-    q_ptr, k_ptr = q.data_ptr(), 0 if k is None else k.data_ptr()
-    cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
-    if not in_place or (q_ptr | k_ptr | cos_ptr | sin_ptr) & 15:
-        if positions is not None:
-            positions = positions.expand(batch, seq).contiguous()
-        return _launch(
-            dense(q), None if k is None else dense(k), _table(cos), _table(sin), positions, layout, transpose
-        )
-    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
-    with at_device(device):
-        status = _native.load().tk_rotary(
-            q_ptr, k_ptr, q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), cos_ptr, sin_ptr,
-            0 if positions is None else positions.data_ptr(), wide, batch, q_heads, kv_heads, seq, head_dim,
-            rotary_dim, rows, q_strides, k_strides, dtype, interleaved, transpose, _stream(q),
-        )
-    _native.check(status, "tk_rotary")
-    _after_launch(q.device)
-    return q_out, k_out
-
-
-class _RotaryFunction(torch.autograd.Function):
-    """Autograd bridge: the backward is the transposed rotation of both gradients in one launch."""
-
-    @staticmethod
-    def forward(ctx: Any, q, k, cos, sin, positions, layout):
-        """Rotate and keep the tables and positions."""
-        ctx.save_for_backward(cos, sin, positions)
-        ctx.layout = layout
-        ctx.set_materialize_grads(False)
-        return _launch(q, k, cos, sin, positions, layout, 0)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, dq, dk):
-        """Input gradients of whichever outputs were used."""
-        cos, sin, positions = ctx.saved_tensors
-        gq = gk = None
-        if dq is not None:
-            gq, gk = _launch(dq, dk, cos, sin, positions, ctx.layout, 1)
-        elif dk is not None:
-            gk, _ = _launch(dk, None, cos, sin, positions, ctx.layout, 1)
-        return gq, gk, None, None, None, None
+    return dense(q), None if k is None else dense(k), table(cos), table(sin), positions
 
 
 def rotary(
@@ -243,6 +162,13 @@ def rotary(
     contiguous (batch, heads, seq, head_dim) tensors; differentiable in ``q``
     and ``k``.
     """
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryFunction.apply(q, k, cos, sin, positions, layout)
-    return _launch(q, k, cos, sin, positions, layout, 0)
+    if layout not in ROTARY_LAYOUTS:
+        raise ValueError(f"rotary layout must be one of {ROTARY_LAYOUTS}")
+    interleaved = layout == "interleaved"
+    out = binding.rotary(q, k, cos, sin, positions, interleaved)
+    if out is None:
+        out = binding.rotary(*_prepare(q, k, cos, sin, positions), interleaved)
+        if out is None:
+            raise ValueError("rotary: unsupported arguments")
+    _after_launch(q.device)
+    return out

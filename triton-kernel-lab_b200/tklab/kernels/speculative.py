@@ -19,14 +19,12 @@ from typing import NamedTuple
 
 import torch
 
-from tklab import _native
-from tklab.kernels._plans import Plans, _after_launch, _stream, at_device, dense, meta, row_strides, stride_array
-from tklab.kernels.flash_attention import _NATIVE_DTYPE
-from tklab.kernels.tree_attention import MAX_TREE_NODES, check_lens, check_parents, in_place
+from tklab._tensors import binding, contiguous, dense, require_cache
+from tklab.kernels.flash_attention import _NATIVE_DTYPE, _after_launch
+from tklab.kernels.tree_attention import MAX_TREE_NODES, check_lens, check_parents
 
-_PROB_TYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_PROB_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 _TOKEN_TYPES = (torch.int32, torch.int64)
-_VERIFY_PLANS, _COMMIT_PLANS = Plans(), Plans()
 
 
 class Verification(NamedTuple):
@@ -37,17 +35,14 @@ class Verification(NamedTuple):
     next_tokens: torch.Tensor  # (batch,), the tokens' dtype
 
 
-def _verify_plan(target_probs, tokens, uniforms, noise, parents, draft_probs, tree_sizes) -> tuple:
-    """Check the contract; return what a call with this metadata passes to the library.
-
-    The first entry says whether every tensor can be read in place.
-    """
+def _prepare_verify(target_probs, tokens, uniforms, noise, parents, draft_probs, tree_sizes) -> tuple:
+    """Check the contract; return the arguments with whatever the kernel cannot read in place copied."""
     if target_probs.ndim != 3 or 0 in target_probs.shape:
         raise ValueError("target_probs must be a non-empty (batch, nodes, vocab) tensor")
     batch, nodes, vocab = target_probs.shape
     if nodes > MAX_TREE_NODES:
         raise ValueError(f"verification supports up to {MAX_TREE_NODES} nodes")
-    if target_probs.dtype not in _PROB_TYPE:
+    if target_probs.dtype not in _PROB_TYPES:
         raise ValueError("target_probs must be float32, bfloat16 or float16")
     if tokens.shape != (batch, nodes) or tokens.dtype not in _TOKEN_TYPES:
         raise ValueError("tokens must be an int32 or int64 tensor of shape (batch, nodes)")
@@ -67,18 +62,15 @@ def _verify_plan(target_probs, tokens, uniforms, noise, parents, draft_probs, tr
         raise ValueError("verification needs its tensors on one device")
     if device.type != "cuda":
         raise ValueError("verification requires CUDA tensors")
-    parent_stride = check_parents(parents, batch, nodes, device)
+    check_parents(parents, batch, nodes, device)
     check_lens(tree_sizes, "tree_sizes", batch, device)
-    drafted = draft_probs is not None and nodes > 1
-    ready = (
-        (target_probs.stride(2) == 1 or vocab == 1)
-        and (not drafted or draft_probs.stride(2) == 1 or vocab == 1)
-        and all(x is None or x.is_contiguous() for x in (tokens, uniforms, noise, parents, tree_sizes))
-    )
+
+    def vocab_contiguous(x: torch.Tensor) -> torch.Tensor:
+        return x if x.stride(2) == 1 else x.contiguous()
+
     return (
-        ready, target_probs.get_device(), stride_array(*target_probs.stride()[:2]), drafted,
-        stride_array(*draft_probs.stride()[:2]) if drafted else None, int(tokens.dtype == torch.int64), parent_stride,
-        batch, nodes, vocab, _PROB_TYPE[target_probs.dtype],
+        vocab_contiguous(target_probs), tokens.contiguous(), uniforms.contiguous(), noise.contiguous(), contiguous(parents),
+        None if draft_probs is None else vocab_contiguous(draft_probs), contiguous(tree_sizes),
     )
 
 
@@ -120,55 +112,27 @@ def verify_draft(
         draft_probs: (batch, nodes - 1, vocab), the type of ``target_probs``.
         tree_sizes: (batch,) int32, nodes in use (0: no path, next token -1).
     """
-    key = (
-        target_probs.shape, target_probs.stride(), target_probs.dtype, target_probs.get_device(), tokens.shape,
-        tokens.stride(), tokens.dtype, tokens.get_device(), uniforms.shape, uniforms.stride(), uniforms.dtype,
-        uniforms.get_device(), noise.shape, noise.stride(), noise.dtype, noise.get_device(), meta(parents),
-        meta(draft_probs), meta(tree_sizes),
-    )
-    plan = _VERIFY_PLANS.get(key) or _VERIFY_PLANS.keep(
-        key, _verify_plan(target_probs, tokens, uniforms, noise, parents, draft_probs, tree_sizes)
-    )
-    (ready, device, target_strides, drafted, draft_strides, wide, parent_stride, batch, nodes, vocab, prob_type) = plan
-    if not ready:
-        return verify_draft(
-            target_probs.contiguous(), tokens.contiguous(), uniforms.contiguous(), noise.contiguous(),
-            parents=None if parents is None else parents.contiguous(),
-            draft_probs=None if draft_probs is None else draft_probs.contiguous(),
-            tree_sizes=None if tree_sizes is None else tree_sizes.contiguous(),
-        )
-    path = torch.empty_like(uniforms, dtype=torch.int32)
-    path_lens = uniforms.new_empty((batch,), dtype=torch.int32)
-    next_tokens = tokens.new_empty((batch,))
-    with at_device(device):
-        status = _native.load().tk_verify_draft(
-            target_probs.data_ptr(), target_strides, draft_probs.data_ptr() if drafted else 0, draft_strides,
-            tokens.data_ptr(), wide, 0 if parents is None else parents.data_ptr(), parent_stride,
-            0 if tree_sizes is None else tree_sizes.data_ptr(), uniforms.data_ptr(), noise.data_ptr(),
-            path.data_ptr(), path_lens.data_ptr(), next_tokens.data_ptr(), batch, nodes, vocab, prob_type,
-            _stream(target_probs),
-        )
-    _native.check(status, "tk_verify_draft")
+    args = (target_probs, tokens, uniforms, noise, parents, draft_probs, tree_sizes)
+    found = binding.verify_draft(*args)
+    if found is None:
+        found = binding.verify_draft(*_prepare_verify(*args))
+        if found is None:
+            raise ValueError("verification: unsupported arguments")
     _after_launch(target_probs.device)
-    return Verification(path, path_lens, next_tokens)
+    return Verification._make(found)
 
 
-def _commit_plan(k_cache, v_cache, k_tree, v_tree, path, path_lens, kv_lens) -> tuple:
-    """Check the contract; return what a call with this metadata passes to the library.
-
-    The first entry says whether every tensor can be read in place.
-    """
+def _prepare_commit(k_cache, v_cache, k_tree, v_tree, path, path_lens, kv_lens) -> tuple:
+    """Check the contract; return the arguments with whatever the kernel cannot read in place copied."""
     if not k_cache.ndim == v_cache.ndim == k_tree.ndim == v_tree.ndim or k_cache.ndim not in (4, 5) or (
         k_cache.shape != v_cache.shape or k_tree.shape != v_tree.shape
     ):
         raise ValueError(
             "K and V caches, and the tree's keys and values, must have identical shapes: ([layers,] batch, heads, rows, dim)"
         )
-    if k_cache.ndim == 4:
-        k_cache, v_cache, k_tree, v_tree = k_cache[None], v_cache[None], k_tree[None], v_tree[None]
-    layers, batch, kv_heads, seq_kv, head_dim = k_cache.shape
-    nodes = k_tree.shape[3]
-    if k_tree.shape != (layers, batch, kv_heads, nodes, head_dim):
+    batch, kv_heads, _, head_dim = k_cache.shape[-4:]
+    nodes = k_tree.shape[-2]
+    if k_tree.shape != (*k_cache.shape[:-4], batch, kv_heads, nodes, head_dim):
         raise ValueError("the caches and the tree disagree on layers, batch, heads or head_dim")
     if 0 in k_cache.shape or nodes == 0:
         raise ValueError("commit does not support empty dimensions")
@@ -188,12 +152,10 @@ def _commit_plan(k_cache, v_cache, k_tree, v_tree, path, path_lens, kv_lens) -> 
         raise ValueError("path must be an int32 tensor of shape (batch, nodes) on the same device")
     check_lens(path_lens, "path_lens", batch, device)
     check_lens(kv_lens, "kv_lens", batch, device)
-    caches = in_place(k_cache, "the K cache") + in_place(v_cache, "the V cache")
-    trees = [row_strides(k_tree), row_strides(v_tree)]
-    ready = None not in trees and all(x.is_contiguous() for x in (path, path_lens, kv_lens))
+    require_cache(k_cache, "the K cache")
+    require_cache(v_cache, "the V cache")
     return (
-        ready, k_cache.get_device(), stride_array(*caches, *trees[0], *trees[1]) if ready else None,
-        layers, batch, kv_heads, nodes, seq_kv, head_dim,
+        k_cache, v_cache, dense(k_tree), dense(v_tree), path.contiguous(), path_lens.contiguous(), kv_lens.contiguous()
     )
 
 
@@ -215,30 +177,11 @@ def commit_draft(
     has no room for are left out, the returned length stops at ``seq_kv`` and
     :func:`tklab.kernels.flash_attention.check_device_status` raises.
     """
-    key = (
-        k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.get_device(), v_cache.shape, v_cache.stride(),
-        v_cache.dtype, v_cache.get_device(), k_tree.shape, k_tree.stride(), k_tree.dtype, k_tree.get_device(),
-        v_tree.shape, v_tree.stride(), v_tree.dtype, v_tree.get_device(), path.shape, path.stride(), path.dtype,
-        path.get_device(), path_lens.shape, path_lens.stride(), path_lens.dtype, path_lens.get_device(), kv_lens.shape,
-        kv_lens.stride(), kv_lens.dtype, kv_lens.get_device(),
-    )
-    plan = _COMMIT_PLANS.get(key) or _COMMIT_PLANS.keep(
-        key, _commit_plan(k_cache, v_cache, k_tree, v_tree, path, path_lens, kv_lens)
-    )
-    ready, device, strides, layers, batch, kv_heads, nodes, seq_kv, head_dim = plan
-    k_ptr, v_ptr, kt_ptr, vt_ptr = k_cache.data_ptr(), v_cache.data_ptr(), k_tree.data_ptr(), v_tree.data_ptr()
-    if (k_ptr | v_ptr) & 15:
-        raise ValueError("the caches need contiguous, 16-byte aligned rows at distinct strides that are multiples of 8")
-    if not ready or (kt_ptr | vt_ptr) & 15:
-        return commit_draft(
-            k_cache, v_cache, dense(k_tree), dense(v_tree), path.contiguous(), path_lens.contiguous(), kv_lens.contiguous()
-        )
-    new_lens = torch.empty_like(kv_lens)
-    with at_device(device):
-        status = _native.load().tk_commit_draft(
-            k_ptr, v_ptr, kt_ptr, vt_ptr, strides, path.data_ptr(), path_lens.data_ptr(), kv_lens.data_ptr(),
-            new_lens.data_ptr(), layers, batch, kv_heads, nodes, seq_kv, head_dim, _stream(k_cache),
-        )
-    _native.check(status, "tk_commit_draft")
+    args = (k_cache, v_cache, k_tree, v_tree, path, path_lens, kv_lens)
+    new_lens = binding.commit_draft(*args)
+    if new_lens is None:
+        new_lens = binding.commit_draft(*_prepare_commit(*args))
+        if new_lens is None:
+            raise ValueError("commit: unsupported arguments")
     _after_launch(k_cache.device)
     return new_lens

@@ -16,24 +16,19 @@ import math
 
 import torch
 
-from tklab import _native
-from tklab.kernels._plans import Plans, _after_launch, _stream, at_device, dense, meta, row_strides, stride_array
-from tklab.kernels.flash_attention import _NATIVE_DTYPE
+from tklab._tensors import binding, contiguous, dense, require_cache
+from tklab.kernels.flash_attention import _NATIVE_DTYPE, _after_launch
 
 MAX_TREE_NODES = 256
 TREE_HEAD_DIMS = tuple(range(8, 129, 8))
 
 
-_PLANS = Plans()
-
-
-def check_parents(parents: torch.Tensor | None, batch: int, nodes: int, device: torch.device) -> int:
-    """Check ``parents`` ((batch, nodes) or (nodes,) int32); return its batch stride (0: one tree for all)."""
+def check_parents(parents: torch.Tensor | None, batch: int, nodes: int, device: torch.device) -> None:
+    """Check optional parents."""
     if parents is None:
-        return 0
+        return
     if parents.dtype != torch.int32 or parents.device != device or parents.shape not in ((batch, nodes), (nodes,)):
         raise ValueError("parents must be an int32 tensor of shape (batch, nodes) or (nodes,) on the same device")
-    return nodes if parents.ndim == 2 else 0
 
 
 def check_lens(lens: torch.Tensor | None, name: str, batch: int, device: torch.device) -> None:
@@ -42,19 +37,8 @@ def check_lens(lens: torch.Tensor | None, name: str, batch: int, device: torch.d
         raise ValueError(f"{name} must be an int32 tensor of shape (batch,) on the same device")
 
 
-def in_place(x: torch.Tensor, name: str) -> tuple[int, ...]:
-    """Strides of a cache, which is never copied."""
-    strides = row_strides(x)
-    if strides is None or any(s == 0 and n > 1 for s, n in zip(strides, x.shape)):
-        raise ValueError(f"{name} needs contiguous, 16-byte aligned rows at distinct strides that are multiples of 8")
-    return strides
-
-
-def _plan(q, k_cache, v_cache, k_tree, v_tree, kv_lens, parents, tree_sizes, scale) -> tuple:
-    """Check the contract; return what a call with this metadata passes to the library.
-
-    The first entry says whether every tensor can be read in place.
-    """
+def _prepare(q, k_cache, v_cache, k_tree, v_tree, kv_lens, parents, tree_sizes, scale) -> tuple:
+    """Check the contract; return the arguments with whatever the kernel cannot read in place copied."""
     if q.ndim != 4 or k_cache.ndim != 4 or k_tree.ndim != 4:
         raise ValueError("q, the caches and the tree's keys and values must be 4-dimensional")
     batch, q_heads, nodes, head_dim = q.shape
@@ -79,25 +63,18 @@ def _plan(q, k_cache, v_cache, k_tree, v_tree, kv_lens, parents, tree_sizes, sca
         raise ValueError("q, keys and values must be on the same device")
     if device.type != "cuda":
         raise ValueError("tree attention requires CUDA tensors")
-    if scale is None:
-        scale = 1.0 / math.sqrt(head_dim)
-    elif not (math.isfinite(scale) and scale > 0.0):
+    if scale is not None and not (math.isfinite(scale) and scale > 0.0):
         raise ValueError("scale must be a positive finite number")
+    if kv_lens is None:
+        raise ValueError("kv_lens is required")
     check_lens(kv_lens, "kv_lens", batch, device)
     check_lens(tree_sizes, "tree_sizes", batch, device)
-    parent_stride = check_parents(parents, batch, nodes, device)
-    caches = in_place(k_cache, "the K cache") + in_place(v_cache, "the V cache")
-    trees = [row_strides(k_tree), row_strides(v_tree)]
-    ready = q.is_contiguous() and None not in trees and all(
-        x is None or x.is_contiguous() for x in (kv_lens, parents, tree_sizes)
-    )
-    with at_device(q.get_device()):
-        ws_bytes = int(
-            _native.load().tk_tree_attn_workspace_bytes(batch, q_heads, kv_heads, nodes, seq_kv, head_dim)
-        )
+    check_parents(parents, batch, nodes, device)
+    require_cache(k_cache, "the K cache")
+    require_cache(v_cache, "the V cache")
     return (
-        ready, q.get_device(), stride_array(*caches, *trees[0], *trees[1]) if ready else None, parent_stride, ws_bytes,
-        batch, q_heads, kv_heads, nodes, seq_kv, head_dim, _NATIVE_DTYPE[dtype], scale,
+        dense(q.contiguous()), k_cache, v_cache, dense(k_tree), dense(v_tree), kv_lens.contiguous(), contiguous(parents),
+        contiguous(tree_sizes), scale,
     )
 
 
@@ -131,38 +108,11 @@ def tree_attention(
     Returns ``o`` shaped like ``q`` (and the base-2 log-sum-exp, scale
     included, (batch, q_heads, nodes) fp32 when ``return_lse``).
     """
-    key = (
-        q.shape, q.stride(), q.dtype, q.get_device(), k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.get_device(),
-        v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.get_device(), k_tree.shape, k_tree.stride(), k_tree.dtype,
-        k_tree.get_device(), v_tree.shape, v_tree.stride(), v_tree.dtype, v_tree.get_device(), kv_lens.shape,
-        kv_lens.stride(), kv_lens.dtype, kv_lens.get_device(), meta(parents), meta(tree_sizes), scale,
-    )
-    plan = _PLANS.get(key) or _PLANS.keep(
-        key, _plan(q, k_cache, v_cache, k_tree, v_tree, kv_lens, parents, tree_sizes, scale)
-    )
-    (ready, device, strides, parent_stride, ws_bytes, batch, q_heads, kv_heads, nodes, seq_kv, head_dim, dtype,
-     scale_value) = plan
-    q_ptr, k_ptr, v_ptr = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    kt_ptr, vt_ptr = k_tree.data_ptr(), v_tree.data_ptr()
-    if (k_ptr | v_ptr) & 15:
-        raise ValueError("the caches need contiguous, 16-byte aligned rows at distinct strides that are multiples of 8")
-    if not ready or (q_ptr | kt_ptr | vt_ptr) & 15:
-        return tree_attention(
-            dense(q.contiguous()), k_cache, v_cache, dense(k_tree), dense(v_tree), kv_lens.contiguous(),
-            None if parents is None else parents.contiguous(),
-            tree_sizes=None if tree_sizes is None else tree_sizes.contiguous(), scale=scale, return_lse=return_lse,
-        )
-    out = torch.empty_like(q)
-    lse = q.new_empty((batch, q_heads, nodes), dtype=torch.float32) if return_lse else None
-    workspace = q.new_empty((ws_bytes,), dtype=torch.uint8)
-    with at_device(device):
-        status = _native.load().tk_tree_attn(
-            q_ptr, k_ptr, v_ptr, kt_ptr, vt_ptr, strides, kv_lens.data_ptr(),
-            0 if parents is None else parents.data_ptr(), parent_stride,
-            0 if tree_sizes is None else tree_sizes.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-            workspace.data_ptr(), ws_bytes, batch, q_heads, kv_heads, nodes, seq_kv, head_dim, dtype, scale_value,
-            _stream(q),
-        )
-    _native.check(status, "tk_tree_attn")
+    args = (q, k_cache, v_cache, k_tree, v_tree, kv_lens, parents, tree_sizes, scale)
+    out = binding.tree_attention(*args, return_lse)
+    if out is None:
+        out = binding.tree_attention(*_prepare(*args), return_lse)
+        if out is None:
+            raise ValueError("tree attention: unsupported arguments")
     _after_launch(q.device)
-    return (out, lse) if return_lse else out
+    return out
