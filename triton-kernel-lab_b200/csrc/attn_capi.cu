@@ -505,12 +505,11 @@ int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree
   a.sms = sm_count();
   if (a.sms <= 0) return tk::kErrNoDriver;
   const int64_t group = q_heads / kv_heads;
-  if (workspace == nullptr ||
-      workspace_bytes < tk::tree_attn_workspace_bytes(batch, kv_heads, group, nodes, seq_kv, head_dim, a.sms))
-    return tk::kErrInvalidArgument;
+  const size_t need = tk::tree_attn_workspace_bytes(batch, kv_heads, group, nodes, seq_kv, head_dim, a.sms);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return tk::kErrInvalidArgument;
   CUtensorMap mq, mk, mv, mkt, mvt;
   if (int rc = make_map(&mq, q, batch * kv_heads, group * nodes, head_dim, dtype,
-                        static_cast<uint32_t>(tk::tree_attn_q_box_rows(group, nodes))))
+                        static_cast<uint32_t>(tk::tree_attn_q_box_rows(batch, kv_heads, group, nodes, seq_kv, head_dim, a.sms))))
     return rc;
   if (int rc = make_map_strided(&mk, k, batch, kv_heads, seq_kv, head_dim, strides, dtype)) return rc;
   if (int rc = make_map_strided(&mv, v, batch, kv_heads, seq_kv, head_dim, strides + 3, dtype)) return rc;

@@ -264,7 +264,7 @@ struct CommitArgs {
 int launch_rotary(const RotaryArgs& a);
 int launch_tree_attn(const TreeAttnArgs& a);
 // Box rows of the query map: 128, or the rows of one copy.
-int tree_attn_q_box_rows(int64_t G, int64_t T);
+int tree_attn_q_box_rows(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms);
 size_t tree_attn_workspace_bytes(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms);
 int launch_verify(const VerifyArgs& a);
 int launch_commit(const CommitArgs& a);

@@ -32,6 +32,13 @@
 // m and l, and tree_attn_combine_kernel joins each row's parts in run order
 // (bitwise reproducible, no atomics).
 //
+// Few items with few tiles are bound by latency, not by bytes: there each item
+// gets a CTA to itself (one launch, no scan, no workspace; TreePlan::whole).
+// Rows are not copied then: joining the copies takes longer than they save on a
+// few tiles.  (Clusters of CTAs that share an item and join it over distributed
+// shared memory were no quicker than the second launch: 12.0 against 12.3 us a
+// call for 8 items of 9 tiles, 24.7 against 22.1 at 256 rows.)
+//
 // Cache rows past kv_lens and tree rows past tree_sizes may hold anything: the
 // scores of masked keys are replaced before they are used, and the rows of a
 // V tile past the last valid key are cleared in shared memory (0 times NaN
@@ -78,7 +85,8 @@ struct TreeCfg {
   static constexpr int kNumBars = 2 * kQBufs + 2 * kStages + 3 * kVStages + 11;
   static constexpr int kCtlOff = kBarOff + kNumBars * 8;
   static constexpr int kMlOff = (kCtlOff + 16 + 32 + 64 + 7) / 8 * 8;  // after control, first segment, scan
-  static constexpr int kSmemBytes = kMlOff + (kEpi ? 2 * kTileRows * 8 : 0);  // m and l of a segment's rows, two buffers
+  // m and l of a segment's rows, two buffers.
+  static constexpr int kSmemBytes = kMlOff + (kEpi ? 2 * kTileRows * 8 : 0);
   static constexpr uint32_t kTmemCols = 512;
   // O of query tile x, or O buffer x, at column x D; the S buffers from here.
   static constexpr uint32_t kColS0 = (kEpi ? 2 : kT) * D;
@@ -156,6 +164,7 @@ struct TreeWalk {
 struct TreePlan {
   int4* cut;
   int by_item;
+  int whole;  // a CTA per item, grid (groups, items): nothing else of the plan or the workspace is used
 };
 
 // One 128-key tile of one row: as the forward's softmax step, with `mask`
@@ -425,6 +434,7 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int wg = warp >> 2;
+  const bool whole_item = kRep == 1 && plan.whole != 0;
   const int group = blockIdx.x;  // rows [group kRows, ...) of every item
 
   uint8_t* sQ = smem;
@@ -447,42 +457,93 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
   int* first = reinterpret_cast<int*>(smem + C::kCtlOff + 16);  // this CTA's run: b, h, u, length; the runs' length
   int* scan = first + 8;                                         // [warps]
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kQBufs; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
+  // Loads of the query rows of a segment (kT tiles of 128 rows, or kRep copies
+  // of 128 / kRep) and of one of its key tiles.
+  auto load_q = [&](const TreeSeg& sg, int qb) {
+    mbar_arrive_expect_tx(&q_full[qb], kT * C::kTileBytes);
+#pragma unroll
+    for (int x = 0; x < kT * kRep; ++x)
+#pragma unroll
+      for (int blk = 0; blk < D / 64; ++blk)
+        tma_load_3d(sQ + (qb * kT + x / kRep) * C::kTileBytes + blk * kBlockBytes +
+                        (x % kRep) * (kTileRows / kRep) * kSwizzleBytes,
+                    &tm_q, &q_full[qb], blk * 64, group * C::kRows + (kRep == 1 ? x * kTileRows : 0),
+                    sg.b * shape.Hkv + sg.h);
+  };
+  auto load_tile = [&](const TreeSeg& sg, int j, bool is_k, int st) {
+    uint64_t* full = is_k ? &k_full[st] : &v_full[st];
+    mbar_arrive_expect_tx(full, C::kTileBytes);
+    const bool on_cache = j < sg.n_cache;
+    const CUtensorMap* map = on_cache ? (is_k ? &tm_k : &tm_v) : (is_k ? &tm_kt : &tm_vt);
+    const int row = (on_cache ? j : j - sg.n_cache) * kTileRows;
+#pragma unroll
+    for (int blk = 0; blk < D / 64; ++blk)
+      tma_load_4d((is_k ? sK : sV) + st * C::kTileBytes + blk * kBlockBytes, map, full, blk * 64, row, sg.h, sg.b);
+  };
+
+  // This CTA's work, by warp 0 alone unless the batch is large, so that it can
+  // also start the first loads before the CTA has met.
+  const bool by_warp = whole_item || shape.B <= 32;
+  uint32_t early = 0;  // K tiles started (warp 0, lane 0)
+  if (warp == 0) {
+    // The lengths first, to cover their latency; the barriers and descriptors a lane each.
+    const int cost = whole_item ? item_cost(shape, blockIdx.y / shape.Hkv)
+                                : by_warp && lane < shape.B ? item_cost(shape, lane) : 0;
+    if (lane == 0) tma_prefetch_map(&tm_q);
+    if (lane == 1) tma_prefetch_map(&tm_k);
+    if (lane == 2) tma_prefetch_map(&tm_kt);
+    if (lane == 3) tma_prefetch_map(&tm_v);
+    if (lane == 4) tma_prefetch_map(&tm_vt);
+    for (int i = lane; i < C::kNumBars; i += 32) {
+      uint64_t* bar = q_full + i;
+      const bool by_warps = (bar >= p_ready && bar < p_ready + 2) || (bar >= o_empty && bar < o_empty + 4);
+      mbar_init(bar, by_warps ? 4 : 1);
     }
-    for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
-    }
-    for (int i = 0; i < C::kVStages; ++i) {
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_ok[i], 1);
-      mbar_init(&v_empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 4);
-      mbar_init(&o_final[i], 1);
-      mbar_init(&o_empty[i], 4);
-      mbar_init(&l_ready[i], 4);
-    }
-    mbar_init(pv_done, 1);
-    ctl->abort = 0;
+    if (lane == 0) ctl->abort = 0;
     fence_mbarrier_init();
-  }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_map(&tm_q);
-    tma_prefetch_map(&tm_k);
-    tma_prefetch_map(&tm_v);
-    tma_prefetch_map(&tm_kt);
-    tma_prefetch_map(&tm_vt);
+    __syncwarp();
+    if (whole_item) {
+      if (lane == 0) {
+        first[0] = blockIdx.y / shape.Hkv;
+        first[1] = blockIdx.y % shape.Hkv;
+        first[2] = 0;
+        first[3] = cost;
+      }
+    } else if (by_warp) {
+      // A run: a scan of the batch's costs, a lane each.
+      const int n = cost;
+      int upto = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, upto, off);
+        if (lane >= off) upto += o;
+      }
+      const int total = __shfl_sync(0xffffffffu, upto, 31) * shape.Hkv;
+      const int run = (total + gridDim.y - 1) / gridDim.y;
+      const int start = blockIdx.y * run, from = (upto - n) * shape.Hkv;
+      if (n > 0 && start >= from && start < from + n * shape.Hkv) {
+        first[0] = lane;
+        first[1] = (start - from) / n;
+        first[2] = (start - from) % n;
+      }
+      if (lane == 0) {
+        first[3] = max(min(run, total - start), 0);
+        first[4] = run;
+      }
+    }
+    __syncwarp();
+    if (by_warp && lane == 0) {
+      TreeWalk ahead{first[0], first[1], first[2], first[3]};
+      TreeSeg sg;
+      if (ahead.next(shape, sg)) {
+        load_q(sg, 0);
+        for (int j = sg.j0; j < sg.j1 && early < C::kStages; ++j, ++early) load_tile(sg, j, true, early);
+      }
+    }
   }
   if (warp == 1) tmem_alloc(&ctl->tmem_base, C::kTmemCols);
-
-  // This CTA's run: a scan of the batch's costs, each thread over consecutive sequences.
-  {
+  if (!by_warp) {
+    // A run: the scan by all threads, each over consecutive sequences.
     const int per = (shape.B + C::kThreads - 1) / C::kThreads;
     const int b0 = min(static_cast<int>(threadIdx.x) * per, shape.B), b1 = min(b0 + per, shape.B);
     int mine = 0;
@@ -535,23 +596,16 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
       // ---------------- TMA producers: warp 0 K, warp 2 V ----------------
       if (lane == 0) {
         const bool is_k = warp == 0;
-        uint8_t* ring = is_k ? sK : sV;
-        uint64_t* full = is_k ? k_full : v_full;
         uint64_t* empty = is_k ? k_empty : v_empty;
+        const uint32_t depth = is_k ? C::kStages : C::kVStages;
         uint32_t g = 0;
         bool ok = true;
         while (ok && walk.next(shape, seg)) {
           for (int j = seg.j0; j < seg.j1; ++j, ++g) {
-            const uint32_t depth = is_k ? C::kStages : C::kVStages;
+            if (is_k && g < early) continue;
             const int st = g % depth;
             if (!(ok = mbar_wait(&empty[st], ((g / depth) & 1) ^ 1, ctl, timeout_ns, status, is_k ? 2 : 3))) break;
-            mbar_arrive_expect_tx(&full[st], C::kTileBytes);
-            const bool on_cache = j < seg.n_cache;
-            const CUtensorMap* map = on_cache ? (is_k ? &tm_k : &tm_v) : (is_k ? &tm_kt : &tm_vt);
-            const int row = (on_cache ? j : j - seg.n_cache) * kTileRows;
-#pragma unroll
-            for (int blk = 0; blk < D / 64; ++blk)
-              tma_load_4d(ring + st * C::kTileBytes + blk * kBlockBytes, map, &full[st], blk * 64, row, seg.h, seg.b);
+            load_tile(seg, j, is_k, st);
           }
         }
       }
@@ -566,17 +620,8 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
             !(ok = warp_wait(&q_empty[qb], ((it / C::kQBufs) & 1) ^ 1, ctl, timeout_ns, status, 1)))
           break;
         if (lane == 0) {
-          mbar_arrive_expect_tx(&q_full[qb], kT * C::kTileBytes);
-          // kT tiles of 128 rows, or kRep copies of 128 / kRep.
-#pragma unroll
-          for (int x = 0; x < kT * kRep; ++x)
-#pragma unroll
-            for (int blk = 0; blk < D / 64; ++blk)
-              tma_load_3d(sQ + (qb * kT + x / kRep) * C::kTileBytes + blk * kBlockBytes +
-                              (x % kRep) * (kTileRows / kRep) * kSwizzleBytes,
-                          &tm_q, &q_full[qb], blk * 64, group * C::kRows + (kRep == 1 ? x * kTileRows : 0),
-                          seg.b * shape.Hkv + seg.h);
-          if (group == 0 && seg.j0 == 0) {
+          if (!by_warp || it > 0) load_q(seg, qb);
+          if (!whole_item && group == 0 && seg.j0 == 0) {
             const bool cut = seg.j1 < seg.n_all;
             const int item = seg.b * shape.Hkv + seg.h;
             const int4 e = cut ? make_int4(item, blockIdx.y, it > 0 ? 1 : 0,
@@ -607,7 +652,7 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
           if (lane == 0) mbar_arrive(&v_ok[st]);
         }
       }
-      if (lane == 0 && group == 0 && !plan.by_item) plan.cut[blockIdx.y] = mine;
+      if (lane == 0 && !whole_item && group == 0 && !plan.by_item) plan.cut[blockIdx.y] = mine;
     } else if (warp == 1) {
       // ---------------- MMA issuer ----------------
       const bool leader = elect_one();
@@ -820,6 +865,7 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
       if (lane == 0) mbar_arrive(&o_empty[ob]);
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   // Now, not earlier: blocks of the joining kernel would sit on SMs where
@@ -959,6 +1005,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
 // The launch: groups of kRows rows x runs, as many CTAs as are resident
 // together (or as the items cost at full caches, if less).
 struct TreeGrid {
+  bool whole;     // a CTA per item (and group)
+  int copies;     // of the rows
   int groups, runs;
   int cuts;  // entries of the plan: items or runs, whichever are fewer
   size_t plan_bytes, ml_bytes, o_bytes;
@@ -967,16 +1015,28 @@ struct TreeGrid {
 constexpr int tree_tiles_per_cta(int64_t R) { return R > kTileRows ? 2 : 1; }
 constexpr int tree_copies(int64_t R) { return R <= 32 ? 4 : R <= 64 ? 2 : 1; }
 
+constexpr int kFewTiles = 5;
+
 TreeGrid tree_grid(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms) {
-  const int64_t group_rows = tree_tiles_per_cta(G * T) * kTileRows / tree_copies(G * T);
-  const int64_t width = D > 64 ? 128 : 64;
-  TreeGrid t;
-  const int64_t groups = (G * T + group_rows - 1) / group_rows;
-  const int64_t tiles = B * Hkv * ((L + kTileRows - 1) / kTileRows + (T + kTileRows - 1) / kTileRows + kItemCost);
-  t.groups = static_cast<int>(groups);
-  t.runs = static_cast<int>(std::max<int64_t>(1, std::min(sms / groups, tiles)));
-  const size_t rows = static_cast<size_t>(groups) * t.runs * 2 * group_rows;
-  t.cuts = static_cast<int>(std::min<int64_t>(B * Hkv, t.runs));
+  const int64_t tile_rows = tree_tiles_per_cta(G * T) * kTileRows, items = B * Hkv;
+  const int64_t item_tiles = (L + kTileRows - 1) / kTileRows + (T + kTileRows - 1) / kTileRows;
+  TreeGrid t{};
+  // A CTA per item, where that is quicker than runs: if an item's tiles take no
+  // longer than the runs' share of all of them and five more, about what the
+  // scan, the second launch and its join cost.
+  const int64_t groups = (G * T + tile_rows - 1) / tile_rows;
+  if (items * groups <= sms && item_tiles <= items * groups * (item_tiles + kItemCost) / sms + kFewTiles) {
+    t.whole = true;
+    t.copies = 1;
+    t.groups = static_cast<int>(groups);
+    return t;
+  }
+  t.copies = tree_copies(G * T);
+  const int64_t group_rows = tile_rows / t.copies, width = D > 64 ? 128 : 64;
+  t.groups = static_cast<int>((G * T + group_rows - 1) / group_rows);
+  t.runs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / t.groups, items * (item_tiles + kItemCost))));
+  const size_t rows = static_cast<size_t>(t.groups) * t.runs * 2 * group_rows;
+  t.cuts = static_cast<int>(std::min<int64_t>(items, t.runs));
   t.plan_bytes = (static_cast<size_t>(t.cuts) * sizeof(int4) + 255) / 256 * 256;
   t.ml_bytes = rows * 8;
   t.o_bytes = rows * static_cast<size_t>(width) * 4;
@@ -1014,14 +1074,15 @@ int launch_tree_t(const TreeAttnArgs& a, const TreeGrid& t) {
                         static_cast<int>(a.Hkv), static_cast<int>(a.T), static_cast<int>(a.L),
                         static_cast<int>(a.G * a.T), static_cast<int>(a.D)};
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
-  const TreePlan plan{reinterpret_cast<int4*>(ws), a.B * a.Hkv <= t.runs ? 1 : 0};
+  const TreePlan plan{reinterpret_cast<int4*>(ws), a.B * a.Hkv <= t.runs ? 1 : 0, t.whole ? 1 : 0};
   float* part_ml = reinterpret_cast<float*>(ws + t.plan_bytes);
   float* part_o = reinterpret_cast<float*>(ws + t.plan_bytes + t.ml_bytes);
-  const dim3 grid(static_cast<unsigned>(t.groups), static_cast<unsigned>(t.runs));
+  const dim3 grid(static_cast<unsigned>(t.groups), static_cast<unsigned>(t.whole ? a.B * a.Hkv : t.runs));
   kern<<<grid, C::kThreads, C::kSmemBytes, a.stream>>>(*a.tm_q, *a.tm_k, *a.tm_v, *a.tm_kt, *a.tm_vt, shape,
                                                       static_cast<uint16_t*>(a.o), a.lse, plan, part_ml, part_o,
                                                       a.scale_log2, a.timeout_ns, a.status);
   if (cudaGetLastError() != cudaSuccess) return kErrLaunch;
+  if (t.whole) return kOk;
   if (t.runs == 1) return kOk;  // nothing is cut
   // An item has about runs / items parts and one: with four or more, warps
   // share a row's parts.
@@ -1033,7 +1094,7 @@ int launch_tree_t(const TreeAttnArgs& a, const TreeGrid& t) {
 
 template <int D, bool kBf16>
 int launch_tree_r(const TreeAttnArgs& a, const TreeGrid& t) {
-  switch (tree_copies(a.G * a.T)) {
+  switch (t.copies) {
     case 4: return launch_tree_t<D, 1, 4, kBf16>(a, t);
     case 2: return launch_tree_t<D, 1, 2, kBf16>(a, t);
     default: break;
@@ -1044,7 +1105,9 @@ int launch_tree_r(const TreeAttnArgs& a, const TreeGrid& t) {
 
 }  // namespace
 
-int tree_attn_q_box_rows(int64_t G, int64_t T) { return kTileRows / tree_copies(G * T); }
+int tree_attn_q_box_rows(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms) {
+  return kTileRows / tree_grid(B, Hkv, G, T, L, D, sms).copies;
+}
 
 size_t tree_attn_workspace_bytes(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms) {
   const TreeGrid t = tree_grid(B, Hkv, G, T, L, D, sms);
