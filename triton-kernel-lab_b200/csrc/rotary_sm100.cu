@@ -20,6 +20,7 @@
 #include <algorithm>
 
 #include "attn_launch.h"
+#include "pdl_launch.h"
 #include "rope_sm100.cuh"
 
 namespace tk {
@@ -55,6 +56,7 @@ constexpr int kRotaryHeads = 4;  // heads in flight
 template <bool kBf16, bool kInterleaved, int W>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryArgs a, int units, int heads_per_block) {
   using C = Chunk<W>;
+  pdl_wait_prerequisites();
   const int chunks = static_cast<int>(a.D) / W, turned = static_cast<int>(a.rotary_dim) / W;
   const long long u = static_cast<long long>(blockIdx.x) * kRotaryThreads + threadIdx.x;
   const long long tok = u / units;  // (b, s)
@@ -176,8 +178,8 @@ int launch_rotary_w(const RotaryArgs& a) {
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>((heads + kRotaryHeads - 1) / kRotaryHeads, 148 * 8 / blocks));
   const int64_t per = (heads + want - 1) / want;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((heads + per - 1) / per));
-  rotary_kernel<kBf16, kInterleaved, W><<<grid, kRotaryThreads, 0, a.stream>>>(a, static_cast<int>(units), static_cast<int>(per));
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+  return launch_pdl(rotary_kernel<kBf16, kInterleaved, W>, grid, dim3(kRotaryThreads), 0, a.stream, 1, a,
+                    static_cast<int>(units), static_cast<int>(per));
 }
 
 // The widest chunk that rotated columns divide into: 16 bytes for the usual

@@ -20,6 +20,7 @@
 // Every node's probability is loaded at once; the walk itself is a warp's, over
 // the visited nodes only.
 #include "attn_launch.h"
+#include "pdl_launch.h"
 #include "sm100_primitives.cuh"
 
 namespace tk {
@@ -123,6 +124,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
   __shared__ unsigned s_filter[kFilterWords];
   __shared__ unsigned long long s_warp[kVerifyThreads / 32], s_best[2][kVerifyMaxCluster];
   cluster_arrive();  // waited for before the first store to another CTA's shared memory
+  pdl_wait_prerequisites();
   const unsigned rank = cluster_rank(), ranks = cluster_size();
   const int64_t b = blockIdx.x / ranks;
   const int T = static_cast<int>(a.T), V = static_cast<int>(a.V);
@@ -330,6 +332,7 @@ constexpr int kCommitHeads = 4;
 // copies it for K and V of all its heads, eight loads in flight; the paths are
 // short, so it is bound by the latency of path, row and store.
 __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const __grid_constant__ CommitArgs a, int chunks, int rows) {
+  pdl_wait_prerequisites();
   const int64_t b = blockIdx.x % a.B, layer = blockIdx.x / a.B;
   const int h0 = blockIdx.y * kCommitHeads, heads = min(kCommitHeads, static_cast<int>(a.H) - h0);
   const int n = min(max(a.path_lens[b], 0), static_cast<int>(a.T));
@@ -370,22 +373,8 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const __grid_con
 
 template <int kType, int N, bool kDraft>
 int launch_verify_t(const VerifyArgs& a, int cluster) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.B * cluster));
-  cfg.blockDim = dim3(kVerifyThreads);
-  cfg.stream = a.stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, verify_kernel<kType, N, kDraft>, a) != cudaSuccess) {
-    cudaGetLastError();
-    return kErrLaunch;
-  }
-  return kOk;
+  return launch_pdl(verify_kernel<kType, N, kDraft>, dim3(static_cast<unsigned>(a.B * cluster)), dim3(kVerifyThreads), 0,
+                    a.stream, cluster, a);
 }
 
 template <int kType>
@@ -419,8 +408,7 @@ int launch_verify(const VerifyArgs& a) {
 int launch_commit(const CommitArgs& a) {
   const int chunks = static_cast<int>(a.D / 8);
   const dim3 grid(static_cast<unsigned>(a.layers * a.B), static_cast<unsigned>((a.H + kCommitHeads - 1) / kCommitHeads));
-  commit_kernel<<<grid, kCommitThreads, 0, a.stream>>>(a, chunks, kCommitThreads / chunks);
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+  return launch_pdl(commit_kernel, grid, dim3(kCommitThreads), 0, a.stream, 1, a, chunks, kCommitThreads / chunks);
 }
 
 }  // namespace tk

@@ -46,6 +46,7 @@
 #include <algorithm>
 
 #include "attn_launch.h"
+#include "pdl_launch.h"
 #include "sm100_primitives.cuh"
 
 namespace tk {
@@ -486,9 +487,7 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
   const bool by_warp = whole_item || shape.B <= 32;
   uint32_t early = 0;  // K tiles started (warp 0, lane 0)
   if (warp == 0) {
-    // The lengths first, to cover their latency; the barriers and descriptors a lane each.
-    const int cost = whole_item ? item_cost(shape, blockIdx.y / shape.Hkv)
-                                : by_warp && lane < shape.B ? item_cost(shape, lane) : 0;
+    // The barriers and descriptors, a lane each; what other kernels may have written from here on.
     if (lane == 0) tma_prefetch_map(&tm_q);
     if (lane == 1) tma_prefetch_map(&tm_k);
     if (lane == 2) tma_prefetch_map(&tm_kt);
@@ -501,6 +500,9 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
     }
     if (lane == 0) ctl->abort = 0;
     fence_mbarrier_init();
+    pdl_wait_prerequisites();
+    const int cost = whole_item ? item_cost(shape, blockIdx.y / shape.Hkv)
+                                : by_warp && lane < shape.B ? item_cost(shape, lane) : 0;
     __syncwarp();
     if (whole_item) {
       if (lane == 0) {
@@ -542,6 +544,7 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
     }
   }
   if (warp == 1) tmem_alloc(&ctl->tmem_base, C::kTmemCols);
+  pdl_wait_prerequisites();
   if (!by_warp) {
     // A run: the scan by all threads, each over consecutive sequences.
     const int per = (shape.B + C::kThreads - 1) / C::kThreads;
@@ -584,6 +587,8 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // (The grid is resident as a whole, so what starts early only waits.)
+  pdl_launch_dependents();
   const uint32_t tmem = ctl->tmem_base;
   TreeWalk walk{first[0], first[1], first[2], first[3]};
   TreeSeg seg;
@@ -868,9 +873,6 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  // Now, not earlier: blocks of the joining kernel would sit on SMs where
-  // this grid still works.
-  pdl_launch_dependents();
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -893,6 +895,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   static_assert(kRows == 1 || kShare == 1, "rows of a warp, or warps of a row");
   constexpr int kPer = D / 32;
   constexpr int kBatch = 8 / kRows;
+  pdl_launch_dependents();
   pdl_wait_prerequisites();
   const int4 cut = plan.cut[blockIdx.y];
   if (cut.x < 0) return;
@@ -1047,21 +1050,9 @@ template <int D, bool kBf16, int kRows, int kShare>
 int launch_tree_combine(const TreeAttnArgs& a, const TreeGrid& t, const TreeShape& shape, const TreePlan& plan,
                         const float* part_ml, const float* part_o, int group_rows) {
   const int64_t per_block = kJoinWarps / kShare * kRows;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((a.G * a.T + per_block - 1) / per_block), static_cast<unsigned>(t.cuts));
-  cfg.blockDim = dim3(32 * kJoinWarps);
-  cfg.stream = a.stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, tree_attn_combine_kernel<D, kBf16, kRows, kShare>, shape, static_cast<uint16_t*>(a.o),
-                         a.lse, plan, part_ml, part_o, t.groups, group_rows) != cudaSuccess) {
-    cudaGetLastError();
-    return kErrLaunch;
-  }
-  return kOk;
+  const dim3 grid(static_cast<unsigned>((a.G * a.T + per_block - 1) / per_block), static_cast<unsigned>(t.cuts));
+  return launch_pdl(tree_attn_combine_kernel<D, kBf16, kRows, kShare>, grid, dim3(32 * kJoinWarps), 0, a.stream, 1, shape,
+                    static_cast<uint16_t*>(a.o), a.lse, plan, part_ml, part_o, t.groups, group_rows);
 }
 
 template <int D, int kT, int kRep, bool kBf16>
@@ -1078,10 +1069,10 @@ int launch_tree_t(const TreeAttnArgs& a, const TreeGrid& t) {
   float* part_ml = reinterpret_cast<float*>(ws + t.plan_bytes);
   float* part_o = reinterpret_cast<float*>(ws + t.plan_bytes + t.ml_bytes);
   const dim3 grid(static_cast<unsigned>(t.groups), static_cast<unsigned>(t.whole ? a.B * a.Hkv : t.runs));
-  kern<<<grid, C::kThreads, C::kSmemBytes, a.stream>>>(*a.tm_q, *a.tm_k, *a.tm_v, *a.tm_kt, *a.tm_vt, shape,
-                                                      static_cast<uint16_t*>(a.o), a.lse, plan, part_ml, part_o,
-                                                      a.scale_log2, a.timeout_ns, a.status);
-  if (cudaGetLastError() != cudaSuccess) return kErrLaunch;
+  if (int rc = launch_pdl(kern, grid, dim3(C::kThreads), C::kSmemBytes, a.stream, 1, *a.tm_q, *a.tm_k, *a.tm_v, *a.tm_kt,
+                          *a.tm_vt, shape, static_cast<uint16_t*>(a.o), a.lse, plan, part_ml, part_o, a.scale_log2,
+                          a.timeout_ns, a.status))
+    return rc;
   if (t.whole) return kOk;
   if (t.runs == 1) return kOk;  // nothing is cut
   // An item has about runs / items parts and one: with four or more, warps
