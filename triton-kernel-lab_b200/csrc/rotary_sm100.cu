@@ -14,9 +14,17 @@
 // Bound by memory: 4 bytes an element and three operations.  A row's angles
 // are fp32 and serve every head, so a thread keeps those of its columns and
 // goes over the heads with them: loading them per head would be twice the
-// data.  A thread has two chunks of W columns, the two sides of its pairs in
-// the half layout, neighbours in the interleaved one or among the copied
-// columns; four heads of loads are in flight before the first is used.
+// data.  A thread has two chunks of W columns: the two sides of its pairs in
+// the half layout, else two half a row apart, so that neighbouring threads
+// have neighbouring chunks (with neighbouring chunks in one thread a request
+// used half of each 32-byte sector it touched).
+//
+// Measured, forward and backward: 113.5 us (6.05 TB/s, 94 % of a copy) for
+// (1, 16384) tokens of 32 + 8 heads of 128, all rotated; 29.6 us (5.1 TB/s)
+// for (3, 2047) tokens of 16 + 16 heads of 96, 24 rotated in neighbouring
+// pairs (36.8 us with neighbouring chunks and 256 threads a CTA).  Forward
+// for 32 x 24 tokens of 32 + 8 heads of 128: 4.3 us, of which 3 us are the
+// latency of one call.
 #include <algorithm>
 
 #include "attn_launch.h"
@@ -50,10 +58,17 @@ __device__ __forceinline__ uint16_t to16(float x) {
   }
 }
 
-constexpr int kRotaryThreads = 256;
-constexpr int kRotaryHeads = 4;  // heads in flight
+// Small CTAs even out the end of a short call: 29.6 us for the (3, 2047)
+// case, 32.4 us with 256 threads.
+constexpr int kRotaryThreads = 128;
+// A thread with at most this many heads has four heads of loads in flight,
+// one with more has two: fewer registers, so more threads an SM, whose loads
+// overlap in place of a thread's own.  With 40 heads a thread 113.5 us with
+// two and 116.7 with four; with 4 heads a thread 34.4 and 31.0 us (3 x 2047
+// tokens, half layout), 4.5 and 4.3 us (32 x 24 tokens).
+constexpr int kFewHeads = 8;
 
-template <bool kBf16, bool kInterleaved, int W>
+template <bool kBf16, bool kInterleaved, int W, int kFlight>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryArgs a, int units, int heads_per_block) {
   using C = Chunk<W>;
   pdl_wait_prerequisites();
@@ -67,15 +82,15 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
   int c1, c2;
   bool turn1, turn2;
   if constexpr (kInterleaved) {
-    c1 = 2 * unit;
-    c2 = c1 + 1;
+    c1 = unit;
+    c2 = unit + (chunks + 1) / 2;
     turn1 = c1 < turned;
     turn2 = c2 < turned;
   } else {
     const int pairs = turned / 2;
     turn1 = turn2 = unit < pairs;
-    c1 = turn1 ? unit : turned + 2 * (unit - pairs);
-    c2 = turn1 ? unit + pairs : c1 + 1;
+    c1 = turn1 ? unit : turned + (unit - pairs);
+    c2 = turn1 ? unit + pairs : c1 + (chunks - turned + 1) / 2;
   }
   const bool has2 = c2 < chunks;
   // Angles of this thread's pairs: W of them (half: the chunks' columns;
@@ -97,8 +112,9 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
 #pragma unroll
         for (int i = 0; i < W; i += 4) {
           if (kInterleaved && i > 0 && !turn2) break;
-          const float4 c = *reinterpret_cast<const float4*>(a.cos + t + i);
-          const float4 v = *reinterpret_cast<const float4*>(a.sin + t + i);
+          const long long o = t + (kInterleaved && i > 0 ? (c2 - c1) * (W / 2) : i);
+          const float4 c = *reinterpret_cast<const float4*>(a.cos + o);
+          const float4 v = *reinterpret_cast<const float4*>(a.sin + o);
           cs[i] = c.x, cs[i + 1] = c.y, cs[i + 2] = c.z, cs[i + 3] = c.w;
           sn[i] = v.x, sn[i + 1] = v.y, sn[i + 2] = v.z, sn[i + 3] = v.w;
         }
@@ -106,8 +122,9 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
 #pragma unroll
         for (int i = 0; i < W; ++i) {
           if (kInterleaved && i >= W / 2 && !turn2) break;
-          cs[i] = a.cos[t + i];
-          sn[i] = a.sin[t + i];
+          const long long o = t + (kInterleaved && i >= W / 2 ? (c2 - c1 - 1) * (W / 2) + i : i);
+          cs[i] = a.cos[o];
+          sn[i] = a.sin[o];
         }
       }
 #pragma unroll
@@ -116,10 +133,10 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
   }
   const int heads = static_cast<int>(a.Hq + a.Hkv);
   const int h_end = min(heads, static_cast<int>(blockIdx.y + 1) * heads_per_block);
-  for (int h0 = blockIdx.y * heads_per_block; h0 < h_end; h0 += kRotaryHeads) {
-    C x1[kRotaryHeads], x2[kRotaryHeads];
+  for (int h0 = blockIdx.y * heads_per_block; h0 < h_end; h0 += kFlight) {
+    C x1[kFlight], x2[kFlight];
 #pragma unroll
-    for (int i = 0; i < kRotaryHeads; ++i) {
+    for (int i = 0; i < kFlight; ++i) {
       const int h = h0 + i;
       if (h >= h_end) break;
       const bool is_q = h < a.Hq;
@@ -130,7 +147,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
       if (has2) x2[i] = *reinterpret_cast<const C*>(x + c2 * W);
     }
 #pragma unroll
-    for (int i = 0; i < kRotaryHeads; ++i) {
+    for (int i = 0; i < kFlight; ++i) {
       const int h = h0 + i;
       if (h >= h_end) break;
       C y1 = x1[i], y2 = x2[i];
@@ -173,13 +190,14 @@ int launch_rotary_w(const RotaryArgs& a) {
   const int64_t heads = a.Hq + a.Hkv;
   const int64_t blocks = (a.B * a.S * units + kRotaryThreads - 1) / kRotaryThreads;
   if (blocks > INT32_MAX) return kErrTooLarge;
-  // All heads in one thread where that fills the device (8 CTAs an SM are
-  // resident), else as few as it takes: short calls are bound by latency.
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>((heads + kRotaryHeads - 1) / kRotaryHeads, 148 * 8 / blocks));
+  // All heads in one thread where that fills the device (16 CTAs an SM), else
+  // as few as it takes: short calls are bound by latency.
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>((heads + 3) / 4, 148 * 16 / blocks));
   const int64_t per = (heads + want - 1) / want;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((heads + per - 1) / per));
-  return launch_pdl(rotary_kernel<kBf16, kInterleaved, W>, grid, dim3(kRotaryThreads), 0, a.stream, 1, a,
-                    static_cast<int>(units), static_cast<int>(per));
+  const bool few = per <= kFewHeads;
+  return launch_pdl(few ? rotary_kernel<kBf16, kInterleaved, W, 4> : rotary_kernel<kBf16, kInterleaved, W, 2>, grid,
+                    dim3(kRotaryThreads), 0, a.stream, 1, a, static_cast<int>(units), static_cast<int>(per));
 }
 
 // The widest chunk that rotated columns divide into: 16 bytes for the usual
