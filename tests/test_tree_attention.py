@@ -277,3 +277,65 @@ def test_rows_past_32_bit_offsets() -> None:
     both = tree_attention(q.repeat(1, 2, 1, 1), cache, cache, tree.repeat(1, 2, 1, 1), tree.repeat(1, 2, 1, 1), lens)
     assert torch.equal(both[:, 2:], o)
     check_device_status()
+
+
+# Rows of one KV head (group x nodes) for every number of copies and tiles of the rows: up to 32, 64, 128, 256 and beyond.
+ROWS = [(1, 1), (4, 8), (3, 11), (8, 8), (5, 13), (8, 16), (3, 43), (8, 32), (1, 200), (5, 77)]
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize(("group", "nodes"), ROWS)
+def test_items_cut_between_ctas(dtype: torch.dtype, dim: int, group: int, nodes: int) -> None:
+    """Caches long enough that a sequence is shared by several CTAs, beside one of a few keys and an empty one."""
+    p = problem(4, 2 * group, 2, nodes, dim, 2600, [2600, 0, 1025, 3], dtype, seed=group + nodes)
+    sizes = torch.tensor([nodes, nodes, max(nodes - 3, 0), nodes // 2], dtype=torch.int32)
+    o, lse = check(p, tree_sizes=sizes)
+    o2, lse2 = tree_attention(**on_gpu(p), tree_sizes=sizes.cuda(), return_lse=True)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("bad", [math.nan, -math.inf])
+@pytest.mark.parametrize(("group", "nodes"), ROWS[1::2])
+def test_unused_rows_of_cut_items_may_hold_anything(bad: float, group: int, nodes: int) -> None:
+    p = problem(3, 2 * group, 2, nodes, 128, 1500, [1400, 0, 515], torch.bfloat16, seed=nodes)
+    sizes = torch.tensor([nodes // 2, nodes, 0], dtype=torch.int32)
+    clean = check(p, tree_sizes=sizes)
+    for b in range(3):
+        for name in ("k", "v"):
+            p[name + "_cache"][b, :, int(p["kv_lens"][b]) :] = bad
+            p[name + "_tree"][b, :, int(sizes[b]) :] = bad
+        p["q"][b, :, int(sizes[b]) :] = bad
+    dirty = tree_attention(**on_gpu(p), tree_sizes=sizes.cuda(), return_lse=True)
+    for a, b in zip(clean, dirty, strict=True):
+        assert torch.equal(a, b)
+    assert bool((dirty[0][2] == 0).all()) and bool(torch.isinf(dirty[1][2]).all())
+    check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize(("group", "nodes"), [(2, 16), (4, 16), (8, 16), (8, 32)])
+def test_more_sequences_than_ctas(group: int, nodes: int) -> None:
+    """Runs of many short items: whole ones inside a run, cut ones at its ends, empty ones between them."""
+    lens = [(53 * i * i + 7 * i) % 400 if i % 5 else 0 for i in range(130)]
+    p = problem(130, 2 * group, 2, nodes, 64, 400, lens, torch.bfloat16, seed=nodes)
+    check(p, tree_sizes=torch.tensor([(3 * i) % (nodes + 1) for i in range(130)], dtype=torch.int32))
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("nodes", [5, 40])
+def test_infinite_cache_rows_in_use(nodes: int) -> None:
+    """An infinite key makes NaN of the rows whose score it makes +inf or NaN, as the formula does, and of no others."""
+    p = problem(2, 4, 2, nodes, 64, 1300, [1300, 1300], torch.float16, seed=6)
+    ref = tree_attention(**on_gpu(p))
+    p["k_cache"][0, 1, 700] = math.inf
+    o = tree_attention(**on_gpu(p))
+    assert bool(torch.isnan(o[0, 2:]).all())
+    assert torch.equal(o[0, :2], ref[0, :2]) and torch.equal(o[1], ref[1])
+    check_device_status()
