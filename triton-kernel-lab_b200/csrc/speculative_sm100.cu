@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
       for (int t = 0; t < tried; ++t) out = out || s_list[t] == v;
       return out;
     };
-    float best = 0.0f, second = 0.0f;
+    float best = 0.0f, second = 0.0f, best_w = 0.0f, best_e = 1.0f;
     int index = -1;
     constexpr int kFlight = N > 1 ? (kDraft ? 2 : 4) : 8;  // steps loaded before any is used
     for (int i0 = first + threadIdx.x; i0 < end; i0 += kVerifyThreads * kFlight) {
@@ -266,11 +266,15 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
         for (int j = 0; j < N; ++j) {
           float r;
           asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e[k][j]));
-          const float score = (kDraft ? p[k][j] - q[k][j] : p[k][j]) * r;
+          const float w = kDraft ? p[k][j] - q[k][j] : p[k][j], score = w * r;
           const bool wins = score > best;
           second = fmaxf(second, wins ? best : score);
           best = wins ? score : best;
           index = wins ? i * N + j : index;
+          if constexpr (kDraft) {
+            best_w = wins ? w : best_w;
+            best_e = wins ? e[k][j] : best_e;
+          }
         }
       }
     }
@@ -283,7 +287,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
       return score > 0.0f && !(skips && was_tried(v)) ? race_key(score, v) : 0ull;
     };
     const bool clear = index < 0 || (second < best * 0.999998f && best < INFINITY);
-    unsigned long long key = clear && index >= 0 ? exact(index) : 0ull;
+    unsigned long long key = 0ull;
+    if (clear && index >= 0) key = kDraft ? race_key(__fdiv_rn(best_w, best_e), index) : exact(index);
     for (unsigned close = __ballot_sync(0xffffffffu, !clear); close != 0; close &= close - 1) {
       for (int i = first + warp * 32 + __ffs(close) - 1 + lane * kVerifyThreads; i < end; i += 32 * kVerifyThreads)
 #pragma unroll
