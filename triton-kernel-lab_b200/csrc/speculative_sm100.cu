@@ -104,8 +104,16 @@ __device__ __forceinline__ void load_probs(const void* p, int64_t i, float (&f)[
 // walks the tree for itself (a few loads; sharing the result would cost a
 // cluster barrier more).  Bound by the row of p (and q) and the noise where
 // there are many sequences, by the chain of dependent loads (tokens, their
-// probabilities, the row) where there are few: the noise, which depends on
-// none, is brought into L2 meanwhile.
+// probabilities, the row) and the walk where there are few.  (Bringing the
+// noise, which depends on none of them, into L2 at the start held up those
+// loads: 30.4 to 27.7 us without it for 128 trees of 64 nodes, 8.5 to 8.3 us
+// for 8.)
+//
+// Measured, per call: 18.3 us for 128 chains of 5 over 50257 float32 entries
+// (4.2 TB/s; 16.0 us, 4.8 TB/s for 50304, whose rows start on 16 bytes);
+// 10.4 us for 32 trees of 64 over 128000 bf16 entries, about 3 us of it the
+// walk; 4.6 us for one chain of 6 over 32000.  With 128 or 256 threads a CTA
+// and more CTAs the first took 18.1 to 19.0 us, the second 11.4 to 15.9.
 //
 // The race is run on w times the hardware reciprocal of e (a few operations an
 // element, no branch); a thread then divides for its own best only, or, if its
@@ -133,9 +141,6 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
   const int steps = (V + N - 1) / N, per = (steps + ranks - 1) / ranks;
   const int first = min(static_cast<int>(rank) * per, steps), end = min(first + per, steps);
   const float* noise = a.noise + b * V;
-  for (int64_t i = static_cast<int64_t>(first) * N + threadIdx.x * 32; i < static_cast<int64_t>(end) * N; i += kVerifyThreads * 32)
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + i));
-
   const int size = a.tree_sizes != nullptr ? min(max(a.tree_sizes[b], 0), T) : T;
   for (int c = threadIdx.x; c < T; c += kVerifyThreads) {
     int n = c - 1;
@@ -240,7 +245,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
     };
     float best = 0.0f, second = 0.0f, best_w = 0.0f, best_e = 1.0f;
     int index = -1;
-    constexpr int kFlight = N > 1 ? (kDraft ? 2 : 4) : 8;  // steps loaded before any is used
+    // Steps loaded before any is used.  N = 1: 18.9 us with 8, 21.5 with 4,
+    // 18.8 with 12 for the 128 chains; N = 4: 10.4 us with 4, 14.3 with 8 for
+    // the 32 trees (fewer CTAs an SM).
+    constexpr int kFlight = N > 1 ? (kDraft ? 2 : 4) : 8;
     for (int i0 = first + threadIdx.x; i0 < end; i0 += kVerifyThreads * kFlight) {
       float p[kFlight][N], q[kFlight][N], e[kFlight][N];
 #pragma unroll
@@ -392,8 +400,9 @@ int launch_verify_n(const VerifyArgs& a, int cluster, bool wide) {
 }  // namespace
 
 int launch_verify(const VerifyArgs& a) {
-  // CTAs of a sequence: one an SM (each walks the tree again), as long as each
-  // has a thread's worth of loads.
+  // CTAs of a sequence: about one an SM (each walks the tree again), as long as
+  // each has a thread's worth of loads.  Two an SM: the same for 32 trees, 22.8
+  // instead of 19.0 us for 128 chains; four: 30.9 us.
   int cluster = 1;
   while (cluster < kVerifyMaxCluster && a.B * cluster < 148 && a.V >= kVerifyThreads * 2 * cluster) cluster *= 2;
   // Four entries a load where every row starts on their boundary.
