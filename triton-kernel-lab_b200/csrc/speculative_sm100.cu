@@ -342,8 +342,10 @@ constexpr int kCommitThreads = 256;
 constexpr int kCommitHeads = 4;
 
 // CTA (b and layer, four heads): a thread has one 16-byte chunk of a row and
-// copies it for K and V of all its heads, eight loads in flight; the paths are
-// short, so it is bound by the latency of path, row and store.
+// copies it for K and V of all its heads, eight loads in flight.  One layer's
+// call is bound by the latency of path, row and store (2.1 us), every layer's
+// by memory: 27.2 us (5.1 TB/s, 79 % of a copy, in pieces of 256 bytes) for 138
+// MB; 27.5 us with two heads a thread, 28.1 with eight.
 __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const __grid_constant__ CommitArgs a, int chunks, int rows) {
   pdl_wait_prerequisites();
   const int64_t b = blockIdx.x % a.B, layer = blockIdx.x / a.B;
