@@ -23,6 +23,9 @@
 // and the copies are joined through shared memory at the end of a segment.  A
 // row's softmax step then takes half or a quarter of the time, which bounds
 // short rows: one warp's 128 columns a row took about 3000 cycles a tile.
+// 24 sequences of 0 to 4096 keys, 16 heads of 64, 5 nodes: 43 us with four
+// copies, 48 with two, 66 with one; 32 sequences of 6144 keys on average, 8
+// heads of 128, 32 rows: 134, 133 and 145 us.
 //
 // Work is cut where the lengths are known, on the device: an item is a (batch,
 // KV head), its work its key tiles, and the items' tiles in one row are
@@ -33,9 +36,9 @@
 // (bitwise reproducible, no atomics).
 //
 // Few items with few tiles are bound by latency, not by bytes: there each item
-// gets a CTA to itself (one launch, no scan, no workspace; TreePlan::whole).
-// Rows are not copied then: joining the copies takes longer than they save on a
-// few tiles.  (Clusters of CTAs that share an item and join it over distributed
+// gets a CTA to itself (one launch, no scan, no workspace; TreePlan::whole,
+// tree_grid).  Rows are not copied then: joining the copies takes longer than
+// they save on a few tiles.  (Clusters of CTAs that share an item and join it over distributed
 // shared memory were no quicker than the second launch: 12.0 against 12.3 us a
 // call for 8 items of 9 tiles, 24.7 against 22.1 at 256 rows.)
 //
@@ -43,6 +46,20 @@
 // scores of masked keys are replaced before they are used, and the rows of a
 // V tile past the last valid key are cleared in shared memory (0 times NaN
 // would be NaN in the product).
+//
+// Measured, per call (cache bytes; useful flops), 32 sequences of 4096 to 8192
+// keys, 8 KV heads of 128, bf16:
+//   32 rows    134 us   6.0 TB/s, 94 % of a copy
+//   256 rows   218 us   3.9 TB/s, 955 TFLOP/s: two tiles' softmax and their
+//              products in turn, the tensor pipe 48 % active, the device at its
+//              power limit (1.45 GHz; 262 us when kept there)
+// and 2 sequences of 100000 to 131000 keys, 4 KV heads of 128, 104 rows, fp16:
+//   87 us      5.4 TB/s, 85 % of a copy.
+// The smallest call (8 items of 1000 keys, 32 rows) takes 9.3 us: two launches
+// and a chain of loads, products and a join.  For 256 rows none of these was
+// quicker: P announced in two parts, so that P V starts under the second
+// part's exponentials (221 us); S and P in halves (232); S read twice, in loops
+// that need fewer registers (227); two softmax warpgroups a tile (315).
 #include <algorithm>
 
 #include "attn_launch.h"
@@ -1018,17 +1035,24 @@ struct TreeGrid {
 constexpr int tree_tiles_per_cta(int64_t R) { return R > kTileRows ? 2 : 1; }
 constexpr int tree_copies(int64_t R) { return R <= 32 ? 4 : R <= 64 ? 2 : 1; }
 
-constexpr int kFewTiles = 5;
-
 TreeGrid tree_grid(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms) {
   const int64_t tile_rows = tree_tiles_per_cta(G * T) * kTileRows, items = B * Hkv;
   const int64_t item_tiles = (L + kTileRows - 1) / kTileRows + (T + kTileRows - 1) / kTileRows;
   TreeGrid t{};
-  // A CTA per item, where that is quicker than runs: if an item's tiles take no
-  // longer than the runs' share of all of them and five more, about what the
-  // scan, the second launch and its join cost.
+  // A CTA per item, where that is quicker than runs: where an item's tiles, one
+  // after another, take no longer than the runs' share of all of them (a CTA's
+  // part of the items' cost) and what cutting the items adds, the plan, the
+  // second launch and its join.  That grows with the rows, and with up to 64
+  // of them runs have copies, which an item alone has not.  us a call, run / a
+  // CTA per item, 8 KV heads of 128:
+  //   32 rows: 1 sequence of 2 cache tiles 8.6 / 8.9, of 4 8.8 / 11.1; 8 of
+  //     them 12.4 / 9.7 and 13.7 / 11.8, 16 of 8 tiles 22.0 / 18.6;
+  //   256 rows: 1 of 2 15.1 / 13.1, of 4 15.6 / 16.6; 4 of 8 25.5 / 24.1, 8 of
+  //     8 30.4 / 25.8.
   const int64_t groups = (G * T + tile_rows - 1) / tile_rows;
-  if (items * groups <= sms && item_tiles <= items * groups * (item_tiles + kItemCost) / sms + kFewTiles) {
+  const bool copied = tree_copies(G * T) > 1;
+  const int64_t share4 = items * groups * (item_tiles + kItemCost) * (copied ? 5 : 9);  // 4 sms x 5/4, or 9/4, of the share
+  if (items * groups <= sms && 4 * item_tiles * sms <= (copied ? 8 : 16) * static_cast<int64_t>(sms) + share4) {
     t.whole = true;
     t.copies = 1;
     t.groups = static_cast<int>(groups);
