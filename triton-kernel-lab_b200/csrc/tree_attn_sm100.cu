@@ -50,7 +50,7 @@
 // Measured, per call (cache bytes; useful flops), 32 sequences of 4096 to 8192
 // keys, 8 KV heads of 128, bf16:
 //   32 rows    134 us   6.0 TB/s, 94 % of a copy
-//   256 rows   218 us   3.9 TB/s, 955 TFLOP/s: two tiles' softmax and their
+//   256 rows   212 us   4.0 TB/s, 980 TFLOP/s: two tiles' softmax and their
 //              products in turn, the tensor pipe 48 % active, the device at its
 //              power limit (1.45 GHz; 262 us when kept there)
 // and 2 sequences of 100000 to 131000 keys, 4 KV heads of 128, 104 rows, fp16:
@@ -204,6 +204,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, int copy, const ui
   float mx[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) mx[i] = -INFINITY;
+  bool live[kBlocks];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) {
     if (kBlocks > 1 && b == kBlocks / 2) {
@@ -211,6 +212,10 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, int copy, const ui
 #pragma unroll
       for (int i = kBlocks / 2; i < kBlocks; ++i) reg_fence(s[i]);
     }
+    // Blocks without a key of any row of the warp: cut tiles and small trees
+    // leave much of a tile empty (80 to 73 us for 336 items of two tiles).
+    live[b] = !kMasked || __any_sync(0xffffffffu, mask[b] != 0u);
+    if (!live[b]) continue;
 #pragma unroll
     for (int c = 0; c < 32; c += 2) {
       if constexpr (kMasked) {
@@ -239,21 +244,23 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, int copy, const ui
   }
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) {
-    uint32_t pk[16];
+    uint32_t pk[16] = {};
+    if (live[b]) {
 #pragma unroll
-    for (int c = 0; c < 32; c += 2) {
-      float x0, x1, p0, p1;
-      f2_unpack(ffma2(f2_pack(__uint_as_float(s[b][c]), __uint_as_float(s[b][c + 1])), scale2, negm2), x0, x1);
-      // Masked tiles keep every exponential on the MUFU so that masked
-      // entries are exactly zero.
-      if (!kMasked && ((c >> 1) & 7) >= 8 - kEmuPairs) {
-        exp2_fma_pair(x0, x1, p0, p1);
-      } else {
-        p0 = ex2(x0);
-        p1 = ex2(x1);
+      for (int c = 0; c < 32; c += 2) {
+        float x0, x1, p0, p1;
+        f2_unpack(ffma2(f2_pack(__uint_as_float(s[b][c]), __uint_as_float(s[b][c + 1])), scale2, negm2), x0, x1);
+        // Masked tiles keep every exponential on the MUFU so that masked
+        // entries are exactly zero.
+        if (!kMasked && ((c >> 1) & 7) >= 8 - kEmuPairs) {
+          exp2_fma_pair(x0, x1, p0, p1);
+        } else {
+          p0 = ex2(x0);
+          p1 = ex2(x1);
+        }
+        sum2[(c >> 1) & 1] = fadd2(sum2[(c >> 1) & 1], f2_pack(p0, p1));
+        pk[c >> 1] = pack2<kBf16>(p0, p1);
       }
-      sum2[(c >> 1) & 1] = fadd2(sum2[(c >> 1) & 1], f2_pack(p0, p1));
-      pk[c >> 1] = pack2<kBf16>(p0, p1);
     }
     tmem_st16(s_addr + (copy * kBlocks + b) * 16, pk);
   }
@@ -293,6 +300,16 @@ __device__ __forceinline__ void tree_mask(const TreeShape& s, int b, int node, i
     const int parent = up[node];
     node = parent < node ? parent : -1;
   }
+}
+
+// Place of 8 columns of a part's row: blocks of four rows, within one the rows'
+// 32 bytes of the same columns side by side.  Threads with a row each then
+// fill whole lines, and a warp of the joining kernel reads four rows as one
+// piece.  (With rows in sequence a store touched a line a lane: 4300 cycles
+// for 256 rows of 128.)
+template <int D>
+__device__ __forceinline__ long long part_at(long long prow, int col) {
+  return (prow >> 2) * (4 * D) + (col >> 3) * 32 + (prow & 3) * 8;
 }
 
 // The end of a segment for one row held by one thread: O from tensor memory
@@ -345,7 +362,7 @@ __device__ __forceinline__ void finish_row(uint32_t o_addr, bool whole, bool liv
       }
       if (row_ok) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) st_global_v8(part_o + prow * D + cb * 32 + q * 8, &o[q * 8]);
+        for (int q = 0; q < 4; ++q) st_global_v8(part_o + part_at<D>(prow, cb * 32 + q * 8), &o[q * 8]);
       }
     }
     if (row_ok) *reinterpret_cast<float2*>(part_ml + prow * 2) = live ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
@@ -420,7 +437,7 @@ __device__ __forceinline__ void finish_copies(bool ok, uint32_t o_addr, int r, b
               make_uint4(pack2<kBf16>(f[0].x * scale, f[0].y * scale), pack2<kBf16>(f[0].z * scale, f[0].w * scale),
                          pack2<kBf16>(f[1].x * scale, f[1].y * scale), pack2<kBf16>(f[1].z * scale, f[1].w * scale));
       } else {
-        float4* dst = reinterpret_cast<float4*>(part_o + (slot_row + jrow) * D + col);
+        float4* dst = reinterpret_cast<float4*>(part_o + part_at<D>(slot_row + jrow, col));
         dst[0] = f[0];
         dst[1] = f[1];
       }
@@ -783,6 +800,11 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
     const int row = group * C::kRows + x * kTileRows + r % kCopyRows;  // of the item's R rows
     const int node = row % shape.T;
     const bool any_row = row - lane < shape.R;  // some row of this warp exists
+    // The bits of a tree of one tile serve all heads of its sequence: the walk to
+    // the root took 3200 of the 14200 cycles of an item of two tiles (80 to 71 us
+    // for 336 of them, 688 rows; 67 with the blocks left out).
+    uint32_t kept[4 / kRep] = {};
+    int kept_b = -1;
     uint32_t g = 0;
     bool ok = true;
     for (int it = 0; ok && walk.next(shape, seg); ++it) {
@@ -795,8 +817,15 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
         uint32_t mask[4 / kRep];
         const bool on_tree = j >= seg.n_cache;
         const int lim = seg.len - j * kTileRows;
-        if (on_tree)
-          tree_mask(shape, seg.b, row < shape.R ? node : size, size, (j - seg.n_cache) * kTileRows + copy * kCopyRows, mask);
+        if (on_tree) {
+          if (seg.b != kept_b || shape.T > kTileRows) {
+            tree_mask(shape, seg.b, row < shape.R ? node : size, size, (j - seg.n_cache) * kTileRows + copy * kCopyRows,
+                      kept);
+            kept_b = seg.b;
+          }
+#pragma unroll
+          for (int i = 0; i < 4 / kRep; ++i) mask[i] = kept[i];
+        }
         if (!(ok = warp_wait(&s_full[buf], (g / kLook) & 1, ctl, timeout_ns, status, 8))) break;
         tc_fence_after();
         if (any_row) {
@@ -902,124 +931,106 @@ constexpr int kJoinWarps = 8;
 // Joins the parts of cut items: with M the largest m,
 // o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over a row's parts in run
 // order.  Bound by the latency of the loads (a row's parts are a few KB, in
-// L2), so each warp keeps eight rows of parts in flight: kRows rows with
-// 8 / kRows parts each, or one row whose parts kShare warps divide.
-template <int D, bool kBf16, int kRows, int kShare>
+// L2): a warp has four rows (part_at: a lane holds columns of one of them) and
+// four parts of each in flight, and kShare warps divide the rows' parts.
+template <int D, bool kBf16, int kShare>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     tree_attn_combine_kernel(const __grid_constant__ TreeShape shape, uint16_t* __restrict__ out,
                              float* __restrict__ lse, TreePlan plan, const float* __restrict__ part_ml,
                              const float* __restrict__ part_o, int groups, int group_rows) {
-  static_assert(kRows == 1 || kShare == 1, "rows of a warp, or warps of a row");
-  constexpr int kPer = D / 32;
-  constexpr int kBatch = 8 / kRows;
+  constexpr int kVec = D / 32;  // float4 of a part's four rows a lane
+  constexpr int kBatch = 4;
   pdl_launch_dependents();
   pdl_wait_prerequisites();
   const int4 cut = plan.cut[blockIdx.y];
   if (cut.x < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int share = warp % kShare;
-  const int row0 = (blockIdx.x * (kJoinWarps / kShare) + warp / kShare) * kRows;
-  float acc[kRows][kPer], m[kRows], l[kRows];
+  const int row0 = (blockIdx.x * (kJoinWarps / kShare) + warp / kShare) * 4;
+  const int row = row0 + ((lane >> 1) & 3);
+  const bool row_ok = row < shape.R;
+  const int group = row0 / group_rows;
+  float m = -INFINITY, l = 0.0f;
+  float4 acc[kVec];
 #pragma unroll
-  for (int k = 0; k < kRows; ++k) {
-    m[k] = -INFINITY;
-    l[k] = 0.0f;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) acc[k][e] = 0.0f;
-  }
+  for (int e = 0; e < kVec; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int p = share; p < cut.w; p += kShare * kBatch) {
-    float2 ml[kRows][kBatch];
-    float v[kRows][kBatch][kPer];
+    float2 ml[kBatch];
+    float4 v[kBatch][kVec];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      const int row = row0 + k;
-      const int group = row / group_rows;
+    for (int i = 0; i < kBatch; ++i) {
+      const int pi = p + i * kShare;
+      ml[i] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int pi = p + i * kShare;
-        ml[k][i] = make_float2(-INFINITY, 0.0f);
+      for (int e = 0; e < kVec; ++e) v[i][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (pi < cut.w && row_ok) {
+        const long long slot = (static_cast<long long>(cut.y + pi) * groups + group) * 2 + (pi == 0 ? cut.z : 0);
+        const long long prow0 = slot * group_rows + row0 % group_rows;
+        ml[i] = *reinterpret_cast<const float2*>(part_ml + (prow0 + (row - row0)) * 2);
+        const float4* src = reinterpret_cast<const float4*>(part_o + prow0 * D) + lane;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) v[k][i][e] = 0.0f;
-        if (pi < cut.w && row < shape.R) {
-          const long long slot = (static_cast<long long>(cut.y + pi) * groups + group) * 2 + (pi == 0 ? cut.z : 0);
-          const long long prow = slot * group_rows + row % group_rows;
-          ml[k][i] = *reinterpret_cast<const float2*>(part_ml + prow * 2);
-          const float* src = part_o + prow * D + lane * kPer;
-          if constexpr (kPer == 4) {
-            const float4 q = *reinterpret_cast<const float4*>(src);
-            v[k][i][0] = q.x, v[k][i][1] = q.y, v[k][i][2] = q.z, v[k][i][3] = q.w;
-          } else {
-            const float2 q = *reinterpret_cast<const float2*>(src);
-            v[k][i][0] = q.x, v[k][i][1] = q.y;
-          }
-        }
+        for (int e = 0; e < kVec; ++e) v[i][e] = src[32 * e];
       }
     }
+    float top = m;
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      float top = m[k];
+    for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[i].x);
+    if (top == -INFINITY) continue;
+    const float keep = ex2(m - top);
+    m = top;
+    l *= keep;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[k][i].x);
-      if (top == -INFINITY) continue;
-      const float keep = ex2(m[k] - top);
-      m[k] = top;
-      l[k] *= keep;
+    for (int e = 0; e < kVec; ++e) acc[e].x *= keep, acc[e].y *= keep, acc[e].z *= keep, acc[e].w *= keep;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) acc[k][e] *= keep;
+    for (int i = 0; i < kBatch; ++i) {
+      const float w = ex2(ml[i].x - top);
+      l += w * ml[i].y;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const float w = ex2(ml[k][i].x - top);
-        l[k] += w * ml[k][i].y;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[k][e] += w * v[k][i][e];
+      for (int e = 0; e < kVec; ++e) {
+        acc[e].x += w * v[i][e].x, acc[e].y += w * v[i][e].y;
+        acc[e].z += w * v[i][e].z, acc[e].w += w * v[i][e].w;
       }
     }
   }
   if constexpr (kShare > 1) {
-    __shared__ float s_acc[kJoinWarps][D];
-    __shared__ float s_ml[kJoinWarps][2];
+    __shared__ float4 s_acc[kJoinWarps][kVec][32];
+    __shared__ float2 s_ml[kJoinWarps][32];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) s_acc[warp][lane * kPer + e] = acc[0][e];
-    if (lane == 0) {
-      s_ml[warp][0] = m[0];
-      s_ml[warp][1] = l[0];
-    }
+    for (int e = 0; e < kVec; ++e) s_acc[warp][e][lane] = acc[e];
+    s_ml[warp][lane] = make_float2(m, l);
     __syncthreads();
     if (share != 0) return;
-    float top = -INFINITY;
+    m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) top = fmaxf(top, s_ml[warp + i][0]);
-    m[0] = top;
-    l[0] = 0.0f;
+    for (int i = 0; i < kShare; ++i) m = fmaxf(m, s_ml[warp + i][lane].x);
+    l = 0.0f;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) acc[0][e] = 0.0f;
-    if (top != -INFINITY) {
+    for (int e = 0; e < kVec; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (m != -INFINITY) {
 #pragma unroll
       for (int i = 0; i < kShare; ++i) {
-        const float w = ex2(s_ml[warp + i][0] - top);
-        l[0] += w * s_ml[warp + i][1];
+        const float2 ml = s_ml[warp + i][lane];
+        const float w = ex2(ml.x - m);
+        l += w * ml.y;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[0][e] += w * s_acc[warp + i][lane * kPer + e];
+        for (int e = 0; e < kVec; ++e) {
+          const float4 v = s_acc[warp + i][e][lane];
+          acc[e].x += w * v.x, acc[e].y += w * v.y, acc[e].z += w * v.z, acc[e].w += w * v.w;
+        }
       }
     }
   }
+  if (!row_ok) return;
+  const long long row_g = static_cast<long long>(cut.x) * shape.R + row;
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-  for (int k = 0; k < kRows; ++k) {
-    const int row = row0 + k;
-    if (row >= shape.R) continue;
-    const long long row_g = static_cast<long long>(cut.x) * shape.R + row;
-    const float inv = l[k] > 0.0f ? 1.0f / l[k] : 0.0f;
-    if (lane * kPer < shape.d_real) {
-      uint16_t* dst = out + row_g * shape.d_real + lane * kPer;
-      if constexpr (kPer == 4) {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<kBf16>(acc[k][0] * inv, acc[k][1] * inv),
-                                                    pack2<kBf16>(acc[k][2] * inv, acc[k][3] * inv));
-      } else {
-        *reinterpret_cast<uint32_t*>(dst) = pack2<kBf16>(acc[k][0] * inv, acc[k][1] * inv);
-      }
-    }
-    if (lse != nullptr && lane == 0) lse[row_g] = l[k] == 0.0f ? -INFINITY : m[k] + lg2(l[k]);
+  for (int e = 0; e < kVec; ++e) {
+    const int col = (4 * e + (lane >> 3)) * 8 + (lane & 1) * 4;
+    if (col < shape.d_real)
+      *reinterpret_cast<uint2*>(out + row_g * shape.d_real + col) =
+          make_uint2(pack2<kBf16>(acc[e].x * inv, acc[e].y * inv), pack2<kBf16>(acc[e].z * inv, acc[e].w * inv));
   }
+  if (lse != nullptr && (lane & 25) == 0) lse[row_g] = l == 0.0f ? -INFINITY : m + lg2(l);
 }
 
 // The launch: groups of kRows rows x runs, as many CTAs as are resident
@@ -1035,6 +1046,8 @@ struct TreeGrid {
 constexpr int tree_tiles_per_cta(int64_t R) { return R > kTileRows ? 2 : 1; }
 constexpr int tree_copies(int64_t R) { return R <= 32 ? 4 : R <= 64 ? 2 : 1; }
 
+constexpr int kFewTiles = 10;
+
 TreeGrid tree_grid(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int64_t D, int sms) {
   const int64_t tile_rows = tree_tiles_per_cta(G * T) * kTileRows, items = B * Hkv;
   const int64_t item_tiles = (L + kTileRows - 1) / kTileRows + (T + kTileRows - 1) / kTileRows;
@@ -1042,17 +1055,19 @@ TreeGrid tree_grid(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int6
   // A CTA per item, where that is quicker than runs: where an item's tiles, one
   // after another, take no longer than the runs' share of all of them (a CTA's
   // part of the items' cost) and what cutting the items adds, the plan, the
-  // second launch and its join.  That grows with the rows, and with up to 64
-  // of them runs have copies, which an item alone has not.  us a call, run / a
-  // CTA per item, 8 KV heads of 128:
-  //   32 rows: 1 sequence of 2 cache tiles 8.6 / 8.9, of 4 8.8 / 11.1; 8 of
-  //     them 12.4 / 9.7 and 13.7 / 11.8, 16 of 8 tiles 22.0 / 18.6;
-  //   256 rows: 1 of 2 15.1 / 13.1, of 4 15.6 / 16.6; 4 of 8 25.5 / 24.1, 8 of
-  //     8 30.4 / 25.8.
+  // second launch and its join: 2 tiles, and with the rows 0 or 3/4 of the share
+  // more (up to 64 rows runs have copies, which an item alone has not).  us a
+  // call, runs / a CTA per item, 8 KV heads of 128:
+  //   32 rows: 1 sequence of 2 cache tiles 8.8 / 8.6, of 4 9.1 / 10.9; 8 of
+  //     2, 4 and 8 11.5 / 9.5, 12.5 / 11.5 and 14.3 / 16.6;
+  //   256 rows: 1 of 2 12.3 / 12.8; 4 of 2 and 8 16.8 / 13.6 and 19.6 / 24.1;
+  //     8 of 4 and 8 25.3 / 17.4 and 28.3 / 25.6.
+  // The host does not see the lengths, and the longest item is what a CTA per
+  // item waits for: only up to kFewTiles (58 sequences of 0 to 1809 keys in a
+  // cache of 2256, 2 KV heads, 150 rows: 32.0 / 36.0).
   const int64_t groups = (G * T + tile_rows - 1) / tile_rows;
-  const bool copied = tree_copies(G * T) > 1;
-  const int64_t share4 = items * groups * (item_tiles + kItemCost) * (copied ? 5 : 9);  // 4 sms x 5/4, or 9/4, of the share
-  if (items * groups <= sms && 4 * item_tiles * sms <= (copied ? 8 : 16) * static_cast<int64_t>(sms) + share4) {
+  const int64_t share4 = items * groups * (item_tiles + kItemCost) * (tree_copies(G * T) > 1 ? 4 : 7);
+  if (items * groups <= sms && item_tiles <= kFewTiles && 4 * item_tiles * sms <= 8 * static_cast<int64_t>(sms) + share4) {
     t.whole = true;
     t.copies = 1;
     t.groups = static_cast<int>(groups);
@@ -1070,12 +1085,12 @@ TreeGrid tree_grid(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int6
   return t;
 }
 
-template <int D, bool kBf16, int kRows, int kShare>
+template <int D, bool kBf16, int kShare>
 int launch_tree_combine(const TreeAttnArgs& a, const TreeGrid& t, const TreeShape& shape, const TreePlan& plan,
                         const float* part_ml, const float* part_o, int group_rows) {
-  const int64_t per_block = kJoinWarps / kShare * kRows;
+  const int64_t per_block = kJoinWarps / kShare * 4;
   const dim3 grid(static_cast<unsigned>((a.G * a.T + per_block - 1) / per_block), static_cast<unsigned>(t.cuts));
-  return launch_pdl(tree_attn_combine_kernel<D, kBf16, kRows, kShare>, grid, dim3(32 * kJoinWarps), 0, a.stream, 1, shape,
+  return launch_pdl(tree_attn_combine_kernel<D, kBf16, kShare>, grid, dim3(32 * kJoinWarps), 0, a.stream, 1, shape,
                     static_cast<uint16_t*>(a.o), a.lse, plan, part_ml, part_o, t.groups, group_rows);
 }
 
@@ -1099,12 +1114,12 @@ int launch_tree_t(const TreeAttnArgs& a, const TreeGrid& t) {
     return rc;
   if (t.whole) return kOk;
   if (t.runs == 1) return kOk;  // nothing is cut
-  // An item has about runs / items parts and one: with four or more, warps
-  // share a row's parts.
+  // An item has about runs / items parts and one: with two or more, warps share
+  // its rows' parts.
   const int64_t parts = t.runs / (a.B * a.Hkv);
-  if (parts >= 16) return launch_tree_combine<D, kBf16, 1, 8>(a, t, shape, plan, part_ml, part_o, C::kRows);
-  if (parts >= 4) return launch_tree_combine<D, kBf16, 1, 2>(a, t, shape, plan, part_ml, part_o, C::kRows);
-  return launch_tree_combine<D, kBf16, 4, 1>(a, t, shape, plan, part_ml, part_o, C::kRows);
+  if (parts >= 8) return launch_tree_combine<D, kBf16, 8>(a, t, shape, plan, part_ml, part_o, C::kRows);
+  if (parts >= 2) return launch_tree_combine<D, kBf16, 2>(a, t, shape, plan, part_ml, part_o, C::kRows);
+  return launch_tree_combine<D, kBf16, 1>(a, t, shape, plan, part_ml, part_o, C::kRows);
 }
 
 template <int D, bool kBf16>
