@@ -339,3 +339,18 @@ def test_infinite_cache_rows_in_use(nodes: int) -> None:
     assert bool(torch.isnan(o[0, 2:]).all())
     assert torch.equal(o[0, :2], ref[0, :2]) and torch.equal(o[1], ref[1])
     check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize(("capacity", "nodes"), [(1300, 5), (1300, 20), (1300, 40), (1300, 100), (200, 5), (200, 100)])
+def test_nan_query_rows_stay_nan(capacity: int, nodes: int) -> None:
+    """A query of NaN has NaN for its output, and no other row does: cut items and items of one CTA."""
+    p = problem(2, 4, 2, nodes, 64, capacity, [capacity, capacity // 3], torch.bfloat16, seed=9)
+    ref = tree_attention(**on_gpu(p))
+    p["q"][0, 1, nodes - 1, 3] = math.nan
+    o, lse = tree_attention(**on_gpu(p), return_lse=True)
+    assert bool(torch.isnan(o[0, 1, nodes - 1]).all()) and bool(torch.isnan(lse[0, 1, nodes - 1]))
+    o[0, 1, nodes - 1] = ref[0, 1, nodes - 1]
+    assert torch.equal(o, ref)
+    check_device_status()

@@ -875,6 +875,7 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
       } else {
         if (!(ok = warp_wait(&o_final[x], it & 1, ctl, timeout_ns, status, 10))) break;
         if (!any_row) continue;
+        if (l_run != l_run) m_run = 0.0f;  // a NaN row stays one
         tc_fence_after();
         const long long slot_row =
             ((static_cast<long long>(blockIdx.y) * gridDim.x + group) * 2 + (it > 0 ? 1 : 0)) * C::kRows;
