@@ -148,6 +148,31 @@ def test_verify_large_vocabularies_and_batches(kind: str) -> None:
 
 @pytest.mark.gpu
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("vocab", [1, 2, 3, 5, 6, 7, 9, 10, 11, 13, 509, 2050, 4101, 20483])
+def test_verify_rows_that_start_anywhere(dtype: torch.dtype, vocab: int) -> None:
+    """Rows of every alignment, in tensors that start and end anywhere in their storage; winners at both ends of a row."""
+    p = draft_of(8, 3, vocab, kind="tree", dtype=dtype, seed=vocab)
+    p["noise"][0::4, 0] = 1e-6
+    p["noise"][1::4, -1] = 1e-6
+    p["noise"][2::4, min(vocab - 1, 3)] = 1e-6
+    ref = check(p)
+    g = on_gpu(p)
+    for before in range(4):
+        target = torch.full((8 * 3 * vocab + before,), math.nan, dtype=dtype, device="cuda")[before:].view(8, 3, vocab)
+        target.copy_(g["target_probs"])
+        noise = torch.full((8 * vocab + 3 - before,), -1.0, device="cuda")[3 - before :].view(8, vocab)
+        noise.copy_(g["noise"])
+        padded = torch.full((8, 3, vocab + 5), math.nan, dtype=dtype, device="cuda")[..., before : before + vocab]
+        padded.copy_(g["target_probs"])
+        for change in ({"target_probs": target}, {"noise": noise}, {"target_probs": padded, "noise": noise}):
+            for a, b in zip(ref, verify_draft(**{**g, **change}), strict=True):
+                assert torch.equal(a, b)
+    check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
 def test_verify_many_nodes_and_sizes() -> None:
     p = draft_of(6, 256, 90, kind="tree", seed=9, sharp=3.0)
     check(p, tree_sizes=torch.tensor([256, 0, 1, 100, -4, 900], dtype=torch.int32))

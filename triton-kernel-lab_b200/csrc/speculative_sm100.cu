@@ -75,16 +75,40 @@ constexpr int kVerifyThreads = 512;
 constexpr int kVerifyMaxCluster = 8;
 constexpr int kFilterWords = 256;
 
-// N consecutive probabilities (or noise values), fp32; vector loads at N = 4.
-template <int kType, int N>
-__device__ __forceinline__ void load_probs(const void* p, int64_t i, float (&f)[N]) {
+// How the vocabulary is read: a thread's step is
+//   kByFour     four entries by a vector load; every row starts on their word;
+//   kByOne      one entry (rows of an odd vocabulary start anywhere);
+//   kCutByFour  four 16-bit entries of such a row, cut out of the two words that
+//               hold them by a shift that is the row's; the steps follow the
+//               noise's words.  At the row's ends, where a word is not all the
+//               row's, entry by entry.
+// By one is bound by its many small requests: 20.1 us against 12.5 cut for 32
+// trees over 128001 bf16 entries, 56 against 30 for 108 over 97835.  With float32
+// or draft probabilities the cut words take registers that loads in flight
+// need: 18.3 us by one, 23.7 cut for the 128 chains below.
+enum { kByFour, kByOne, kCutByFour };
+
+// Entries [i, i + N) of the row from p[at], whose first is `shift` past a word.
+template <int kType, int N, bool kShifted>
+__device__ __forceinline__ void load_step(const void* p, int64_t at, int i, int shift, float (&f)[N]) {
   if constexpr (N == 1) {
-    f[0] = prob_at<kType>(p, i);
+    f[0] = prob_at<kType>(p, at + i);
   } else if constexpr (kType == kProbF32) {
-    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + i);
     f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
   } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    const uint16_t* x = static_cast<const uint16_t*>(p) + at + i;
+    uint2 v;
+    if constexpr (!kShifted) {
+      v = *reinterpret_cast<const uint2*>(x);
+    } else {
+      const uint2* w = reinterpret_cast<const uint2*>(x - shift);
+      const uint2 lo = w[0], hi = w[1];
+      const bool two = shift & 2;
+      const uint32_t a0 = two ? lo.y : lo.x, a1 = two ? hi.x : lo.y, a2 = two ? hi.y : hi.x;
+      v.x = __funnelshift_r(a0, a1, (shift & 1) * 16);
+      v.y = __funnelshift_r(a1, a2, (shift & 1) * 16);
+    }
     const uint32_t u[2] = {v.x, v.y};
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -98,6 +122,13 @@ __device__ __forceinline__ void load_probs(const void* p, int64_t i, float (&f)[
       }
     }
   }
+}
+
+// Entries between p[at] and the word of four that it is in.
+template <int kType>
+__device__ __forceinline__ int word_shift(const void* p, int64_t at) {
+  constexpr int kBytes = kType == kProbF32 ? 4 : 2;
+  return static_cast<int>((reinterpret_cast<uintptr_t>(p) + at * kBytes) / kBytes % 4);
 }
 
 // One cluster per sequence, its CTAs over the vocabulary.  Every CTA of it
@@ -122,8 +153,10 @@ __device__ __forceinline__ void load_probs(const void* p, int64_t i, float (&f)[
 // of the rounded quotients.  Dividing wherever a
 // thread's or a warp's best so far might be beaten bound it: B = 32, 128000
 // entries, bf16, 24 to 45 us.
-template <int kType, int N, bool kDraft>
+template <int kType, int kRead, bool kDraft>
 __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_constant__ VerifyArgs a) {
+  constexpr int N = kRead == kByOne ? 1 : 4;
+  constexpr bool kShifted = kRead == kCutByFour;
   __shared__ int s_parent[kTreeMaxNodes], s_path[kTreeMaxNodes];
   __shared__ long long s_token[kTreeMaxNodes], s_list[kTreeMaxNodes];
   __shared__ float s_prob[kTreeMaxNodes], s_uniform[kTreeMaxNodes];
@@ -137,10 +170,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
   const int64_t b = blockIdx.x / ranks;
   const int T = static_cast<int>(a.T), V = static_cast<int>(a.V);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // This CTA's part of the vocabulary, in steps of N.
-  const int steps = (V + N - 1) / N, per = (steps + ranks - 1) / ranks;
-  const int first = min(static_cast<int>(rank) * per, steps), end = min(first + per, steps);
   const float* noise = a.noise + b * V;
+  // This CTA's part of the vocabulary, in steps of N: step i has the entries
+  // from N i - lead on.
+  const int lead = kShifted ? word_shift<kProbF32>(noise, 0) : 0;
+  const int steps = (V + lead + N - 1) / N, per = (steps + ranks - 1) / ranks;
+  const int first = min(static_cast<int>(rank) * per, steps), end = min(first + per, steps);
   const int size = a.tree_sizes != nullptr ? min(max(a.tree_sizes[b], 0), T) : T;
   for (int c = threadIdx.x; c < T; c += kVerifyThreads) {
     int n = c - 1;
@@ -207,7 +242,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
     // A filter over the steps that hold a tried token.
     for (int t = lane; !kDraft && t < tried; t += 32)
       if (s_list[t] >= 0 && s_list[t] < V) {
-        const unsigned i = static_cast<unsigned>(s_list[t]) / N;
+        const unsigned i = (static_cast<unsigned>(s_list[t]) + lead) / N;
         atomicOr(&s_filter[(i >> 5) % kFilterWords], 1u << (i & 31));
       }
     if (lane == 0) {
@@ -234,6 +269,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
   const int last = s_path[length - 1];
   const int64_t row = b * a.target_stride[0] + last * a.target_stride[1];
   const int64_t drow = kDraft ? b * a.draft_stride[0] + last * a.draft_stride[1] : 0;
+  const int shift = kShifted ? (word_shift<kType>(a.target, row) + 4 - lead) % 4 : 0;  // of the steps in p
   for (int attempt = 0; attempt < 2; ++attempt) {
     const bool residual = attempt == 0 && tried > 0;
     const bool minus = kDraft && residual;
@@ -245,30 +281,36 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
     };
     float best = 0.0f, second = 0.0f, best_w = 0.0f, best_e = 1.0f;
     int index = -1;
-    // Steps loaded before any is used.  N = 1: 18.9 us with 8, 21.5 with 4,
-    // 18.8 with 12 for the 128 chains; N = 4: 10.4 us with 4, 14.3 with 8 for
-    // the 32 trees (fewer CTAs an SM).
-    constexpr int kFlight = N > 1 ? (kDraft ? 2 : 4) : 8;
+    // Steps loaded before any is used.  By one: 18.9 us with 8, 21.5 with 4,
+    // 18.8 with 12 for the 128 chains; by four: 10.4 us with 4, 14.3 with 8 for
+    // the 32 trees (fewer CTAs an SM); cut: the same with 2 and 4.
+    constexpr int kFlight = kRead == kByOne ? 8 : kDraft || kShifted ? 2 : 4;
     for (int i0 = first + threadIdx.x; i0 < end; i0 += kVerifyThreads * kFlight) {
       float p[kFlight][N], q[kFlight][N], e[kFlight][N];
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
-        const int i = i0 + k * kVerifyThreads;
+        const int i = i0 + k * kVerifyThreads, v = i * N - lead;
 #pragma unroll
         for (int j = 0; j < N; ++j) p[k][j] = q[k][j] = 0.0f, e[k][j] = 1.0f;
         if (i < end) {
-          load_probs<kType, N>(a.target, row + static_cast<int64_t>(i) * N, p[k]);
-          load_probs<kProbF32, N>(noise, static_cast<int64_t>(i) * N, e[k]);
-          if (minus) load_probs<kType, N>(a.draft, drow + static_cast<int64_t>(i) * N, q[k]);
+          if (kShifted && (v < shift || v + 8 > V)) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              if (v + j >= 0 && v + j < V) p[k][j] = prob_at<kType>(a.target, row + v + j), e[k][j] = noise[v + j];
+          } else {
+            load_step<kType, N, kShifted>(a.target, row, v, shift, p[k]);
+            load_step<kProbF32, N, false>(noise, 0, v, 0, e[k]);
+            if (minus) load_step<kType, N, false>(a.draft, drow, v, 0, q[k]);
+          }
         }
       }
 #pragma unroll
       for (int k = 0; k < kFlight; ++k) {
-        const int i = i0 + k * kVerifyThreads;
+        const int i = i0 + k * kVerifyThreads, v = i * N - lead;
         if (skips && ((s_filter[(i >> 5) % kFilterWords] >> (i & 31)) & 1u)) {
 #pragma unroll
           for (int j = 0; j < N; ++j)
-            if (was_tried(i * N + j)) p[k][j] = 0.0f;
+            if (was_tried(v + j)) p[k][j] = 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
@@ -278,7 +320,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
           const bool wins = score > best;
           second = fmaxf(second, wins ? best : score);
           best = wins ? score : best;
-          index = wins ? i * N + j : index;
+          index = wins ? v + j : index;
           if constexpr (kDraft) {
             best_w = wins ? w : best_w;
             best_e = wins ? e[k][j] : best_e;
@@ -301,7 +343,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const __grid_
       for (int i = first + warp * 32 + __ffs(close) - 1 + lane * kVerifyThreads; i < end; i += 32 * kVerifyThreads)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-          const unsigned long long mine = exact(i * N + j);
+          const int v = i * N - lead + j;
+          const unsigned long long mine = v >= 0 && v < V ? exact(v) : 0ull;
           key = mine > key ? mine : key;
         }
     }
@@ -386,17 +429,19 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const __grid_con
   }
 }
 
-template <int kType, int N, bool kDraft>
+template <int kType, int kRead, bool kDraft>
 int launch_verify_t(const VerifyArgs& a, int cluster) {
-  return launch_pdl(verify_kernel<kType, N, kDraft>, dim3(static_cast<unsigned>(a.B * cluster)), dim3(kVerifyThreads), 0,
-                    a.stream, cluster, a);
+  static_assert(kRead != kCutByFour || (kType != kProbF32 && !kDraft), "16-bit probabilities alone are cut");
+  return launch_pdl(verify_kernel<kType, kRead, kDraft>, dim3(static_cast<unsigned>(a.B * cluster)), dim3(kVerifyThreads),
+                    0, a.stream, cluster, a);
 }
 
 template <int kType>
 int launch_verify_n(const VerifyArgs& a, int cluster, bool wide) {
   if (a.draft != nullptr)
-    return wide ? launch_verify_t<kType, 4, true>(a, cluster) : launch_verify_t<kType, 1, true>(a, cluster);
-  return wide ? launch_verify_t<kType, 4, false>(a, cluster) : launch_verify_t<kType, 1, false>(a, cluster);
+    return wide ? launch_verify_t<kType, kByFour, true>(a, cluster) : launch_verify_t<kType, kByOne, true>(a, cluster);
+  return wide ? launch_verify_t<kType, kByFour, false>(a, cluster)
+              : launch_verify_t<kType, kType == kProbF32 ? kByOne : kCutByFour, false>(a, cluster);
 }
 
 }  // namespace
@@ -407,7 +452,7 @@ int launch_verify(const VerifyArgs& a) {
   // instead of 19.0 us for 128 chains; four: 30.9 us.
   int cluster = 1;
   while (cluster < kVerifyMaxCluster && a.B * cluster < 148 && a.V >= kVerifyThreads * 2 * cluster) cluster *= 2;
-  // Four entries a load where every row starts on their boundary.
+  // Whether every row starts on a word of four.
   const uintptr_t bytes = a.type == kProbF32 ? 16 : 8;
   bool wide = a.V % 4 == 0 && a.target_stride[0] % 4 == 0 && a.target_stride[1] % 4 == 0 &&
               reinterpret_cast<uintptr_t>(a.target) % bytes == 0 && reinterpret_cast<uintptr_t>(a.noise) % 16 == 0;
