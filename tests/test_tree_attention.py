@@ -354,3 +354,11 @@ def test_nan_query_rows_stay_nan(capacity: int, nodes: int) -> None:
     o[0, 1, nodes - 1] = ref[0, 1, nodes - 1]
     assert torch.equal(o, ref)
     check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize(("group", "capacity"), [(80, 1500), (80, 200), (160, 1400)])
+def test_more_groups_of_rows_than_runs(group: int, capacity: int) -> None:
+    """Rows in so many groups that each has one run, and in more groups than the device has SMs."""
+    check(problem(2, group, 1, 256, 64, capacity, [capacity, 130], torch.bfloat16, seed=group))

@@ -54,10 +54,10 @@
 //              products in turn, the tensor pipe 48 % active, the device at its
 //              power limit (1.45 GHz; 262 us when kept there)
 // and 2 sequences of 100000 to 131000 keys, 4 KV heads of 128, 104 rows, fp16:
-//   87 us      5.4 TB/s, 85 % of a copy.
-// The smallest call (8 items of 1000 keys, 32 rows) takes 9.3 us: two launches
+//   84 us      5.6 TB/s, 88 % of a copy.
+// The smallest call (8 items of 1000 keys, 32 rows) takes 9.2 us: two launches
 // and a chain of loads, products and a join.  For 256 rows none of these was
-// quicker: P announced in two parts, so that P V starts under the second
+// quicker than 218 to 223 us at the time: P announced in two parts, so that P V starts under the second
 // part's exponentials (221 us); S and P in halves (232); S read twice, in loops
 // that need fewer registers (227); two softmax warpgroups a tile (315).
 #include <algorithm>
