@@ -19,6 +19,8 @@
 //
 // Every node's probability is loaded at once; the walk itself is a warp's, over
 // the visited nodes only.
+#include <algorithm>
+
 #include "attn_launch.h"
 #include "pdl_launch.h"
 #include "sm100_primitives.cuh"
@@ -467,9 +469,12 @@ int launch_verify(const VerifyArgs& a) {
 }
 
 int launch_commit(const CommitArgs& a) {
+  // No more threads than a tree's rows have chunks: a CTA is short, and smaller
+  // ones are more an SM (trees of 8, every layer: 8.1 us instead of 10.2).
   const int chunks = static_cast<int>(a.D / 8);
+  const int threads = static_cast<int>(std::min<int64_t>(kCommitThreads, (a.T * chunks + 31) / 32 * 32));
   const dim3 grid(static_cast<unsigned>(a.layers * a.B), static_cast<unsigned>((a.H + kCommitHeads - 1) / kCommitHeads));
-  return launch_pdl(commit_kernel, grid, dim3(kCommitThreads), 0, a.stream, 1, a, chunks, kCommitThreads / chunks);
+  return launch_pdl(commit_kernel, grid, dim3(threads), 0, a.stream, 1, a, chunks, threads / chunks);
 }
 
 }  // namespace tk
