@@ -362,3 +362,18 @@ def test_nan_query_rows_stay_nan(capacity: int, nodes: int) -> None:
 def test_more_groups_of_rows_than_runs(group: int, capacity: int) -> None:
     """Rows in so many groups that each has one run, and in more groups than the device has SMs."""
     check(problem(2, group, 1, 256, 64, capacity, [capacity, 130], torch.bfloat16, seed=group))
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize(("group", "nodes"), [(1, 1), (4, 8), (3, 11), (8, 8), (8, 16)])
+@pytest.mark.parametrize("capacity", [300, 1300, 2600])
+def test_nan_key_beside_large_scores(group: int, nodes: int, capacity: int) -> None:
+    """Scores of some hundreds: whatever part of a row has the NaN weighs nothing beside the others, and the row is NaN."""
+    p = problem(2, 2 * group, 2, nodes, 64, capacity, [capacity, capacity // 2], torch.bfloat16, seed=nodes, spread=100.0)
+    ref = tree_attention(**on_gpu(p))
+    p["k_cache"][0, 1, 140] = math.nan
+    o, lse = tree_attention(**on_gpu(p), return_lse=True)
+    assert bool(torch.isnan(o[0, group:]).all()) and bool(torch.isnan(lse[0, group:]).all())
+    assert torch.equal(o[0, :group], ref[0, :group]) and torch.equal(o[1], ref[1])
+    check_device_status()

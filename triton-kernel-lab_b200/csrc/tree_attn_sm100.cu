@@ -320,7 +320,7 @@ __device__ __forceinline__ void finish_row(uint32_t o_addr, bool whole, bool liv
                                            float* part_ml, float* part_o) {
   if (whole) {
     const bool wide_store = (d_real % 16) == 0 && (reinterpret_cast<uintptr_t>(out) & 31u) == 0;
-    const float inv = (live && l > 0.0f) ? 1.0f / l : 0.0f;
+    const float inv = (live && l != 0.0f) ? 1.0f / l : 0.0f;  // of a NaN: NaN
     uint16_t* orow = out + row_g * d_real;
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb) {
@@ -395,7 +395,9 @@ __device__ __forceinline__ void finish_copies(bool ok, uint32_t o_addr, int r, b
     const float2 e = ml[i * kCopyRows + jrow];
     if (e.x != -INFINITY) jl += ex2(e.x - jtop) * e.y;
   }
-  const float scale = whole ? (jl > 0.0f ? 1.0f / jl : 0.0f) : 1.0f;
+  // (A sum of NaN makes NaN of its row, also where the copy that it is from
+  // weighs nothing beside the others and its O is left out.)
+  const float scale = whole ? (jl != 0.0f ? 1.0f / jl : 0.0f) : 1.0f;
   const bool jrow_ok = ok && jrow < R;
 #pragma unroll
   for (int pass = 0; pass < D / 64; ++pass) {
@@ -1023,7 +1025,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   }
   if (!row_ok) return;
   const long long row_g = static_cast<long long>(cut.x) * shape.R + row;
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // of a NaN: NaN
 #pragma unroll
   for (int e = 0; e < kVec; ++e) {
     const int col = (4 * e + (lane >> 3)) * 8 + (lane & 1) * 4;
