@@ -377,3 +377,34 @@ def test_nan_key_beside_large_scores(group: int, nodes: int, capacity: int) -> N
     assert bool(torch.isnan(o[0, group:]).all()) and bool(torch.isnan(lse[0, group:]).all())
     assert torch.equal(o[0, :group], ref[0, :group]) and torch.equal(o[1], ref[1])
     check_device_status()
+
+
+def assert_attends_like(o, lse, ref):
+    """:func:`assert_attends` where the formula is finite; the same infinities and NaN where it is not (of the
+    log-sum-exp: none that is finite, for a score of +inf makes it +inf and the kernel's NaN)."""
+    ref_o, ref_lse, spread = ref
+    got, got_lse = o.double().cpu(), lse.double().cpu()
+    odd = ~torch.isfinite(ref_o)
+    assert torch.equal(torch.nan_to_num(got[odd], nan=0.0), torch.nan_to_num(ref_o[odd], nan=0.0))
+    lost = torch.isnan(ref_lse) | (ref_lse == math.inf)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref_o)) and torch.equal(torch.isnan(got_lse) | (got_lse == math.inf), lost)
+    put = lambda x, at: torch.where(at, torch.zeros_like(x), x)  # noqa: E731
+    assert_attends(put(got, odd).to(o.dtype), put(got_lse, lost).float(), (put(ref_o, odd), put(ref_lse, lost), put(spread, odd)))
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize(("group", "nodes"), [(3, 11), (8, 8), (3, 43), (8, 32)])
+@pytest.mark.parametrize("capacity", [300, 1800])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_keys_that_are_not_finite_count_at_every_column(dtype, dim, group, nodes, capacity, bad) -> None:
+    """One entry of a key, at eight columns of a whole tile, items of one CTA and cut ones: a score of NaN or +inf makes
+    NaN of its row as the formula does, whatever the rows' number, and one of -inf takes the key out."""
+    p = problem(8, group, 1, nodes, dim, capacity, [capacity] * 8, dtype, seed=dim + nodes)
+    for b, column in enumerate((0, 3, 4, 7, 8, 11, 12, 15)):
+        p["k_cache"][b, 0, 128 + column, 5] = bad
+    o, lse = tree_attention(**on_gpu(p), return_lse=True)
+    assert_attends_like(o, lse, tree_attention_reference(**p))
+    check_device_status()

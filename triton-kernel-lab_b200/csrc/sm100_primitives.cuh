@@ -550,6 +550,13 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
+// The same, NaN if one of them is.
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Pack two floats into one 32-bit word of 16-bit values, `lo` in bits 0..15
 // (the even K element of a tcgen05 A operand pair).
 template <bool kBf16>

@@ -185,13 +185,23 @@ struct TreePlan {
   int whole;  // a CTA per item, grid (groups, items): nothing else of the plan or the workspace is used
 };
 
+// The maximum; with kNan NaN if one of them is.
+template <bool kNan>
+__device__ __forceinline__ float tile_max(float a, float b, float c) {
+  return kNan ? fmax3_nan(a, b, c) : fmax3(a, b, c);
+}
+
 // One 128-key tile of one row: as the forward's softmax step, with `mask`
 // (kMasked) a bit per key.  With copies (kRep > 1) only copy `copy`'s 128 /
-// kRep keys; P of the others is zero.
+// kRep keys; P of the others is zero.  The polynomial exponentials
+// (kEmuPairs) take any NaN or -inf for 2^-126, so where they run the tile's
+// maximum carries NaN, a row whose maximum is NaN or +inf (the formula's inf -
+// inf) gets a sum of NaN, and one with only -inf so far a sum of 0.
 template <bool kBf16, bool kMasked, int kEmuPairs, int kRep>
 __device__ __forceinline__ void softmax_tile(uint32_t s_addr, int copy, const uint32_t (&mask)[4 / kRep], float scale_log2,
                                              float& m_run, float& l_run, float& alpha, bool& need) {
   constexpr int kBlocks = 4 / kRep;  // 32-key blocks
+  constexpr bool kEmulates = !kMasked && kEmuPairs > 0;
   uint32_t s[kBlocks][32];
   const uint32_t own = s_addr + copy * (32 * kBlocks);
 #pragma unroll
@@ -222,11 +232,11 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, int copy, const ui
         if (!((mask[b] >> c) & 1u)) s[b][c] = __float_as_uint(-INFINITY);
         if (!((mask[b] >> (c + 1)) & 1u)) s[b][c + 1] = __float_as_uint(-INFINITY);
       }
-      mx[(c >> 1) & 7] = fmax3(mx[(c >> 1) & 7], __uint_as_float(s[b][c]), __uint_as_float(s[b][c + 1]));
+      mx[(c >> 1) & 7] = tile_max<kEmulates>(mx[(c >> 1) & 7], __uint_as_float(s[b][c]), __uint_as_float(s[b][c + 1]));
     }
   }
-  const float mxa = fmax3(mx[0], mx[1], mx[2]), mxb = fmax3(mx[3], mx[4], mx[5]);
-  const float m_tile = fmax3(mxa, mxb, fmaxf(mx[6], mx[7]));
+  const float mxa = tile_max<kEmulates>(mx[0], mx[1], mx[2]), mxb = tile_max<kEmulates>(mx[3], mx[4], mx[5]);
+  const float m_tile = tile_max<kEmulates>(mxa, mxb, tile_max<kEmulates>(mx[6], mx[7], mx[7]));
   const float m_new = fmaxf(m_run, m_tile * scale_log2);
   need = m_new > m_run + kTreeRescale;
   const float m_use = need ? m_new : m_run;
@@ -252,7 +262,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, int copy, const ui
         f2_unpack(ffma2(f2_pack(__uint_as_float(s[b][c]), __uint_as_float(s[b][c + 1])), scale2, negm2), x0, x1);
         // Masked tiles keep every exponential on the MUFU so that masked
         // entries are exactly zero.
-        if (!kMasked && ((c >> 1) & 7) >= 8 - kEmuPairs) {
+        if (kEmulates && ((c >> 1) & 7) >= 8 - kEmuPairs) {
           exp2_fma_pair(x0, x1, p0, p1);
         } else {
           p0 = ex2(x0);
@@ -268,6 +278,10 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, int copy, const ui
   f2_unpack(sum2[0], sa0, sa1);
   f2_unpack(sum2[1], sb0, sb1);
   l_run = l_run * alpha + ((sa0 + sa1) + (sb0 + sb1));
+  if constexpr (kEmulates) {
+    if (!(m_tile < INFINITY)) l_run = __uint_as_float(0x7fffffffu);
+    if (m_use == -INFINITY && l_run == l_run) l_run = 0.0f;
+  }
   m_run = m_use;
 }
 
