@@ -256,7 +256,8 @@ TK_API int tk_rotary(const void* q, const void* k, void* q_out, void* k_out, con
  *                   lse = -inf
  *   lse             (batch, q_heads, nodes) fp32 base-2 log-sum-exp, or NULL
  * Node t attends the valid cache rows, its ancestors and itself.  Cache rows
- * past kv_lens and tree rows past tree_sizes may hold anything, NaN included.
+ * past kv_lens, tree rows past tree_sizes and, for a node, the rows of nodes
+ * that it does not attend may hold anything, NaN included.
  * head_dim a multiple of 8 up to 128.  `workspace`: at least
  * tk_tree_attn_workspace_bytes(...) bytes, 256-byte aligned, private to this
  * call until it completes (NULL when that is 0). */

@@ -408,3 +408,29 @@ def test_keys_that_are_not_finite_count_at_every_column(dtype, dim, group, nodes
     o, lse = tree_attention(**on_gpu(p), return_lse=True)
     assert_attends_like(o, lse, tree_attention_reference(**p))
     check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 120])
+@pytest.mark.parametrize(("group", "nodes"), ROWS[1:])
+@pytest.mark.parametrize("capacity", [200, 1500])
+@pytest.mark.parametrize("tree", [False, True])
+def test_values_of_other_nodes_may_hold_anything(dtype, dim, group, nodes, capacity, tree) -> None:
+    """Entries of drafted values that are not finite reach the nodes that attend them, as the formula has it, and no others."""
+    p = problem(3, 2 * group, 2, nodes, dim, capacity, [capacity, 0, 77], dtype, seed=nodes + dim, tree=tree)
+    clean = tree_attention(**on_gpu(p), return_lse=True)
+    for b in range(3):
+        for h in range(2):
+            at = torch.randperm(nodes, generator=torch.Generator().manual_seed(2 * b + h))[: 3 if nodes > 3 else 1].tolist()
+            for node, bad, column in zip(at, (math.nan, math.inf, -math.inf), (5, dim - 1, 8), strict=False):
+                p["v_tree"][b, h, node, column] = bad
+    p["v_tree"][2, 1, nodes - 1] = math.nan
+    o, lse = tree_attention(**on_gpu(p), return_lse=True)
+    ref_o = tree_attention_reference(**p)[0]
+    fine = torch.isfinite(ref_o).cuda()
+    assert torch.equal(o[fine], clean[0][fine]) and torch.equal(lse, clean[1])
+    got, want = o.double().cpu()[~fine.cpu()], ref_o[~fine.cpu()]
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+    check_device_status()

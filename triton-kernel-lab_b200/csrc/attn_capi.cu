@@ -523,6 +523,8 @@ int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree
   a.kv_lens = kv_lens;
   a.parents = parents;
   a.tree_sizes = tree_sizes;
+  a.v_tree = v_tree;
+  for (int i = 0; i < 3; ++i) a.v_tree_stride[i] = strides[9 + i];
   a.o = o;
   a.lse = lse;
   a.parent_stride = parent_stride;

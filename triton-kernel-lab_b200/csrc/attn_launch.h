@@ -206,6 +206,8 @@ struct TreeAttnArgs {
   const int* kv_lens;     // (B)
   const int* parents;     // (B or 1, T), or nullptr: a chain
   const int* tree_sizes;  // (B), or nullptr: T each
+  const void* v_tree;     // (B, Hkv, T, D) at v_tree_stride, as in tm_vt
+  int64_t v_tree_stride[3];
   void* o;                // (B, Hkv * G, T, D)
   float* lse;             // (B, Hkv * G, T), or nullptr
   int64_t parent_stride;  // T, or 0 for one tree shared by all sequences

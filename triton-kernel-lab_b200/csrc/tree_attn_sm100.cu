@@ -42,10 +42,13 @@
 // shared memory were no quicker than the second launch: 12.0 against 12.3 us a
 // call for 8 items of 9 tiles, 24.7 against 22.1 at 256 rows.)
 //
-// Cache rows past kv_lens and tree rows past tree_sizes may hold anything: the
-// scores of masked keys are replaced before they are used, and the rows of a
-// V tile past the last valid key are cleared in shared memory (0 times NaN
-// would be NaN in the product).
+// Cache rows past kv_lens, tree rows past tree_sizes and, for a row, nodes that
+// it does not attend may hold anything: the scores of masked keys are replaced
+// before they are used, and in shared memory a V tile's rows past the last valid
+// key are cleared, and in tree tiles what is not finite (0 times it would be NaN
+// in the product); the rows that attend the latter get it added at the end.
+// (With copies an infinite value of a cache row, which every row attends, makes
+// NaN instead of infinity.)
 //
 // Measured, per call (cache bytes; useful flops), 32 sequences of 4096 to 8192
 // keys, 8 KV heads of 128, bf16:
@@ -124,6 +127,8 @@ struct TreeShape {
   const int* tree_sizes;
   const int* parents;
   long long parent_stride;
+  const uint16_t* v_tree;  // the tree's values, at element strides
+  long long v_batch, v_head, v_row;
   int B, Hkv, T, L, R;  // R = G T query rows per KV head
   int d_real;
 };
@@ -316,6 +321,72 @@ __device__ __forceinline__ void tree_mask(const TreeShape& s, int b, int node, i
   }
 }
 
+template <bool kBf16>
+__device__ __forceinline__ float half_value(uint16_t h) {
+  if constexpr (kBf16) {
+    return __uint_as_float(static_cast<uint32_t>(h) << 16);
+  } else {
+    return __half2float(__ushort_as_half(h));
+  }
+}
+
+// The halves of a word that hold no finite number, as bits 15 and 31: their
+// exponents are all ones, and one more carries into the sign's place.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t kExp = kBf16 ? 0x7f807f80u : 0x7c007c00u, kOne = kBf16 ? 0x00800080u : 0x04000400u;
+  return ((w & kExp) + kOne) & 0x80008000u;
+}
+
+// The larger magnitudes of two words' halves, NaN before all.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t w) {
+  if constexpr (kBf16) {
+    const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), __habs2(*reinterpret_cast<__nv_bfloat162*>(&w)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  } else {
+    const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&a), __habs2(*reinterpret_cast<__half2*>(&w)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+}
+
+// Clears what is not finite in the first `rows` rows of a V tile (one warp) and
+// returns whether there was anything.  The search is a packed maximum a word:
+// one warp has the whole tile to look at while others make its P.
+template <int D, bool kBf16>
+__device__ __forceinline__ bool clear_not_finite(uint8_t* tile, int rows, int lane) {
+  constexpr int kFlight = 2;
+  uint32_t top[kFlight] = {};
+#pragma unroll 1
+  for (int off = lane * 16; off < rows * kSwizzleBytes; off += kFlight * 32 * 16) {
+    uint4 v[D / 64][kFlight];
+#pragma unroll
+    for (int blk = 0; blk < D / 64; ++blk)
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i)  // (past the rows: loaded still, not looked at)
+        v[blk][i] = *reinterpret_cast<const uint4*>(tile + blk * kBlockBytes + min(off + i * 32 * 16, kBlockBytes - 16));
+#pragma unroll
+    for (int blk = 0; blk < D / 64; ++blk)
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i)
+        if (off + i * 32 * 16 < rows * kSwizzleBytes)
+          top[i] = larger<kBf16>(larger<kBf16>(larger<kBf16>(larger<kBf16>(top[i], v[blk][i].x), v[blk][i].y), v[blk][i].z),
+                                 v[blk][i].w);
+  }
+  uint32_t found = 0;
+#pragma unroll
+  for (int i = 0; i < kFlight; ++i) found |= not_finite<kBf16>(top[i]);
+  if (!__any_sync(0xffffffffu, found != 0)) return false;
+#pragma unroll 1
+  for (int blk = 0; blk < D / 64; ++blk)
+#pragma unroll 1
+    for (int off = lane * 4; off < rows * kSwizzleBytes; off += 32 * 4) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(tile + blk * kBlockBytes + off);
+      *w &= ~((not_finite<kBf16>(*w) >> 15) * 0xffffu);
+    }
+  return true;
+}
+
 // Place of 8 columns of a part's row: blocks of four rows, within one the rows'
 // 32 bytes of the same columns side by side.  Threads with a row each then
 // fill whole lines, and a warp of the joining kernel reads four rows as one
@@ -383,6 +454,47 @@ __device__ __forceinline__ void finish_row(uint32_t o_addr, bool whole, bool liv
   }
 }
 
+// Adds to columns [c0, c1) of a row that this thread has stored (as output, or
+// as a part's row) the values that are not finite of the nodes in the segment's
+// tree tiles that the row's node attends.  What was stored lacks them: in the
+// product they would make NaN of every row, 0 times infinity, and not of those
+// that attend them only.
+template <int D, bool kBf16>
+__device__ __forceinline__ void add_not_finite(const TreeShape& s, const TreeSeg& seg, int node, int c0, int c1, bool whole,
+                                               uint16_t* out_row, float* part_o, long long prow) {
+  const int lo = max(seg.j0 - seg.n_cache, 0) * kTileRows, hi = (seg.j1 - seg.n_cache) * kTileRows;
+  const uint16_t* v = s.v_tree + seg.b * s.v_batch + seg.h * s.v_head;
+  if (hi <= 0) return;
+  asm volatile("" ::: "memory");  // after the stores, which were of other types
+#pragma unroll 1
+  for (int n = node; n >= lo;) {
+    if (n < hi) {
+#pragma unroll 1
+      for (int c = c0; c < min(c1, s.d_real); ++c) {
+        const uint16_t x = v[n * s.v_row + c];
+        if (not_finite<kBf16>(x) == 0) continue;
+        if (whole) {
+          uint16_t* o = out_row + c;
+          *o = static_cast<uint16_t>(pack2<kBf16>(half_value<kBf16>(*o) + half_value<kBf16>(x), 0.0f));
+        } else {
+          part_o[part_at<D>(prow, c & ~7) + (c & 7)] += half_value<kBf16>(x);
+        }
+      }
+    }
+    const int parent = s.parents != nullptr ? s.parents[seg.b * s.parent_stride + n] : n - 1;
+    n = parent < n ? parent : -1;
+  }
+}
+
+// Out of line for the epilogue warpgroup: a call that is hardly ever made, and
+// whose code would delay the smallest ones (8.9 us, 9.2 with it in line).  With
+// two tiles in line: there a call costs the softmax warps registers (53 us, 54).
+template <int D, bool kBf16>
+__device__ __noinline__ void call_add_not_finite(const TreeShape& s, const TreeSeg& seg, int node, int c0, int c1, bool whole,
+                                                 uint16_t* out_row, float* part_o, long long prow) {
+  add_not_finite<D, kBf16>(s, seg, node, c0, c1, whole, out_row, part_o, prow);
+}
+
 // The end of a segment whose rows are held as kRep copies: thread r holds row
 // r % (128 / kRep) of copy r / (128 / kRep).  64 columns at a time, each row
 // weighted by 2^(m - M) goes to shared memory (16-byte chunks XORed with the
@@ -390,8 +502,10 @@ __device__ __forceinline__ void finish_row(uint32_t o_addr, bool whole, bool liv
 // call it; `ok` only skips the work.
 template <int D, int kRep, bool kBf16>
 __device__ __forceinline__ void finish_copies(bool ok, uint32_t o_addr, int r, bool whole, const float2* ml, float4* join,
-                                              int R, long long item_row, long long slot_row, int d_real, uint16_t* out,
-                                              float* lse, float* part_ml, float* part_o) {
+                                              const TreeShape& shape, const TreeSeg& seg, bool patch, long long item_row,
+                                              long long slot_row, uint16_t* out, float* lse, float* part_ml,
+                                              float* part_o) {
+  const int R = shape.R, d_real = shape.d_real;
   constexpr int kCopyRows = kTileRows / kRep;
   constexpr int kCols = 64 / kRep;
   const int mrow = r % kCopyRows;  // the row it writes
@@ -459,6 +573,10 @@ __device__ __forceinline__ void finish_copies(bool ok, uint32_t o_addr, int r, b
       }
     }
   }
+  if (patch && jrow_ok && jl != 0.0f)
+    for (int c = jpart * kCols; c < D; c += 64)
+      call_add_not_finite<D, kBf16>(shape, seg, jrow % shape.T, c, c + kCols, whole, out + (item_row + jrow) * d_real,
+                                    part_o, slot_row + jrow);
   if (jrow_ok && jpart == 0) {
     if (!whole)
       *reinterpret_cast<float2*>(part_ml + (slot_row + jrow) * 2) = make_float2(jtop, jl);
@@ -505,6 +623,9 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
   uint64_t* l_ready = o_empty + 2;          // [2]: m and l of O buffer's segment written
   uint64_t* pv_done = l_ready + 2;          // with two S buffers: P V of every tile
   CtaControl* ctl = reinterpret_cast<CtaControl*>(smem + C::kCtlOff);
+  // Values that are not finite were taken out of a tree tile of this CTA.  Warp 3
+  // sets it before v_ok of the tile, which the softmax warps wait for.
+  volatile int* patched = reinterpret_cast<int*>(smem + C::kCtlOff + sizeof(CtaControl));
   int* first = reinterpret_cast<int*>(smem + C::kCtlOff + 16);  // this CTA's run: b, h, u, length; the runs' length
   int* scan = first + 8;                                         // [warps]
 
@@ -548,7 +669,10 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
       const bool by_warps = (bar >= p_ready && bar < p_ready + 2) || (bar >= o_empty && bar < o_empty + 4);
       mbar_init(bar, by_warps ? 4 : 1);
     }
-    if (lane == 0) ctl->abort = 0;
+    if (lane == 0) {
+      ctl->abort = 0;
+      *patched = 0;
+    }
     fence_mbarrier_init();
     pdl_wait_prerequisites();
     const int cost = whole_item ? item_cost(shape, blockIdx.y / shape.Hkv)
@@ -701,9 +825,13 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
             for (int blk = 0; blk < D / 64; ++blk)
               for (int off = from + lane * 16; off < kBlockBytes; off += 32 * 16)
                 *reinterpret_cast<uint4*>(sV + st * C::kTileBytes + blk * kBlockBytes + off) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-            __syncwarp();
           }
+          // Not every row attends a tree row: what is not finite is taken out
+          // (and added where it belongs at the segment's end).
+          const bool odd = jt >= 0 && clear_not_finite<D, kBf16>(sV + st * C::kTileBytes, min(max(valid, 0), kTileRows), lane);
+          if (odd && lane == 0) *patched = 1;
+          if (odd || valid < kTileRows) fence_proxy_async_smem();
+          __syncwarp();
           if (lane == 0) mbar_arrive(&v_ok[st]);
         }
       }
@@ -874,6 +1002,9 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
           }
           tmem_wait_st();
         }
+        // (P V needs the tile's V anyhow; before p_ready, so that v_ok cannot be a
+        // phase further.)
+        if (on_tree && !(ok = warp_wait(&v_ok[g % C::kVStages], (g / C::kVStages) & 1, ctl, timeout_ns, status, 16))) break;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[buf]);
@@ -898,6 +1029,10 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
         finish_row<D, kBf16>(o_addr, seg.j0 == 0 && seg.j1 == seg.n_all, live, row < shape.R, m_run, l_run,
                              (static_cast<long long>(seg.b) * shape.Hkv + seg.h) * shape.R + row,
                              slot_row + x * kTileRows + r, shape.d_real, out, lse, part_ml, part_o);
+        if (*patched && live && row < shape.R)
+          add_not_finite<D, kBf16>(shape, seg, node, 0, D, seg.j0 == 0 && seg.j1 == seg.n_all,
+                                   out + ((static_cast<long long>(seg.b) * shape.Hkv + seg.h) * shape.R + row) * shape.d_real,
+                                   part_o, slot_row + x * kTileRows + r);
       }
     }
   } else {
@@ -922,11 +1057,14 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
       const float2* ml = reinterpret_cast<const float2*>(smem + C::kMlOff) + ob * kTileRows;
       if constexpr (kRep > 1) {
         finish_copies<D, kRep, kBf16>(ok, t_lane + D * ob, r, whole, ml, reinterpret_cast<float4*>(smem + C::kJoinOff),
-                                      shape.R, item_row, slot_row, shape.d_real, out, lse, part_ml, part_o);
+                                      shape, seg, *patched != 0, item_row, slot_row, out, lse, part_ml, part_o);
       } else if (ok && group * C::kRows + r - lane < shape.R) {
         const int row = group * C::kRows + r;
         finish_row<D, kBf16>(t_lane + D * ob, whole, ml[r].y != 0.0f, row < shape.R, ml[r].x, ml[r].y, item_row + row,
                              slot_row + r, shape.d_real, out, lse, part_ml, part_o);
+        if (*patched && ml[r].y != 0.0f && row < shape.R)
+          call_add_not_finite<D, kBf16>(shape, seg, row % shape.T, 0, D, whole, out + (item_row + row) * shape.d_real,
+                                        part_o, slot_row + r);
       }
       tc_fence_before();
       __syncwarp();
@@ -1117,7 +1255,8 @@ int launch_tree_t(const TreeAttnArgs& a, const TreeGrid& t) {
   static_assert(C::kSmemBytes <= 232448, "shared memory exceeds the sm_100 limit");
   auto kern = tree_attn_kernel<D, kT, kRep, kBf16>;
   if (int rc = prepare_kernel(reinterpret_cast<const void*>(kern), C::kSmemBytes, C::kLaunchRegs, nullptr)) return rc;
-  const TreeShape shape{a.kv_lens, a.tree_sizes, a.parents, a.parent_stride, static_cast<int>(a.B),
+  const TreeShape shape{a.kv_lens, a.tree_sizes, a.parents, a.parent_stride, static_cast<const uint16_t*>(a.v_tree),
+                        a.v_tree_stride[0], a.v_tree_stride[1], a.v_tree_stride[2], static_cast<int>(a.B),
                         static_cast<int>(a.Hkv), static_cast<int>(a.T), static_cast<int>(a.L),
                         static_cast<int>(a.G * a.T), static_cast<int>(a.D)};
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);

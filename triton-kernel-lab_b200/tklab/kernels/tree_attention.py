@@ -98,7 +98,7 @@ def tree_attention(
             multiple of 8 up to 128, float16 or bfloat16.
         k_cache, v_cache: (batch, kv_heads, seq_kv, head_dim), any strides with
             contiguous 16-byte aligned rows; rows past ``kv_lens`` may hold anything.
-        k_tree, v_tree: (batch, kv_heads, nodes, head_dim).
+        k_tree, v_tree: (batch, kv_heads, nodes, head_dim); for a node, the rows that it does not attend may hold anything.
         kv_lens: (batch,) int32, valid cache rows.
         parents: (batch, nodes) or (nodes,) int32, ``parents[t] < t`` (anything
             else makes ``t`` a root); None: a chain.
