@@ -434,3 +434,31 @@ def test_values_of_other_nodes_may_hold_anything(dtype, dim, group, nodes, capac
     got, want = o.double().cpu()[~fine.cpu()], ref_o[~fine.cpu()]
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
     check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize(("group", "nodes"), [(1, 1), (4, 8), (8, 8), (8, 16), (8, 32)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_small_weights_beside_a_large_one(group: int, nodes: int, dtype: torch.dtype) -> None:
+    """4000 keys at 2^-25.5 of the one that dominates, whose own value is 0: they are the output.  So many sequences that
+    few items are cut.  In float16 a weight is rounded to a multiple of 2^-31 of the largest at worst."""
+    count, dim, batch = 4000, 64, 160
+    p = problem(1, group, 1, nodes, dim, count + 1, [count + 1], dtype, seed=nodes, tree=False)
+    for name in ("q", "k_cache", "k_tree", "v_tree"):
+        p[name].zero_()
+    p["q"][..., 0] = 1.0
+    p["k_cache"][..., 0] = -25.5 * math.log(2.0)
+    p["k_tree"][..., 0] = -60.0
+    p["v_cache"] = ((p["v_cache"].float().abs() + 0.5) * 64.0).to(dtype)
+    p["k_cache"][:, :, 0] = 0.0
+    p["v_cache"][:, :, 0] = 0.0
+    many = {n: None if t is None else t.cuda().repeat(batch, *[1] * (t.ndim - 1)) for n, t in p.items()}
+    o, lse = tree_attention(**many, scale=1.0, return_lse=True)
+    ref_o, ref_lse, spread = tree_attention_reference(**p, scale=1.0)
+    largest = float(p["v_cache"].abs().max())
+    bound = (2.0 * ROUND[dtype] + 2.0**-12) * spread + (count * 2.0**-32 * largest if dtype == torch.float16 else 0.0)
+    err = (o.double().cpu() - ref_o).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+    assert torch.allclose(lse.double().cpu(), ref_lse.expand(batch, -1, -1), atol=2e-4)
+    check_device_status()

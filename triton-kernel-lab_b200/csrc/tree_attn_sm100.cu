@@ -113,7 +113,14 @@ struct TreeCfg {
   static constexpr uint32_t kColS0 = (kEpi ? 2 : kT) * D;
 };
 
-constexpr float kTreeRescale = 8.0f;  // as the forward's: P stays below 2^8, O is rescaled rarely
+constexpr float kTreeRescale = 8.0f;  // as the forward's: P stays below 2^8 (2^15 in float16), O is rescaled rarely
+// float16 has nothing below 2^-24: there exponents are taken from 7 below a
+// row's maximum (m is that everywhere below), so that a weight is lost from P V
+// only under 2^-32 of the largest.  (Taken from the maximum, it was lost under
+// 2^-25: thousands of such keys were missing in O, though not in the sum, where
+// the largest's own value was small.)  bfloat16 has float32's exponents.
+template <bool kBf16>
+constexpr float kTreeRaise = kBf16 ? 0.0f : 7.0f;
 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, CtaControl* ctl, uint64_t timeout_ns,
                                           int* status, int site) {
@@ -242,7 +249,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_addr, int copy, const ui
   }
   const float mxa = tile_max<kEmulates>(mx[0], mx[1], mx[2]), mxb = tile_max<kEmulates>(mx[3], mx[4], mx[5]);
   const float m_tile = tile_max<kEmulates>(mxa, mxb, tile_max<kEmulates>(mx[6], mx[7], mx[7]));
-  const float m_new = fmaxf(m_run, m_tile * scale_log2);
+  const float m_new = fmaxf(m_run, kBf16 ? m_tile * scale_log2 : fmaf(m_tile, scale_log2, -kTreeRaise<kBf16>));
   need = m_new > m_run + kTreeRescale;
   const float m_use = need ? m_new : m_run;
   alpha = (m_run == -INFINITY) ? 0.0f : ex2(m_run - m_use);
