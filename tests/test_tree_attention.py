@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+from conftest import load_selftest_lib
 from oracle.speculative_oracle import tree_attention_reference
 from tklab import _native
 from tklab.kernels.flash_attention import check_device_status
@@ -102,6 +103,18 @@ def test_library_refuses_before_launch(kwargs: dict, status: int) -> None:
             "stream": None}
     args.update(kwargs)
     assert _native.load().tk_tree_attn(*args.values()) == status
+
+
+def test_joining_takes_entries_of_cut_items_only() -> None:
+    """Whatever an entry holds where a CTA gave up, no part past the runs' and no row past the items' is touched."""
+    ok = load_selftest_lib().tk_selftest_tree_cut_ok
+    big = 2**31 - 1
+    for item, run, slot, parts, good in [
+        (0, 0, 0, 1, 1), (11, 0, 1, 148, 1), (5, 147, 1, 1, 1), (-1, 0, 0, 0, 0), (12, 0, 0, 1, 0), (0, 148, 0, 1, 0),
+        (0, -1, 0, 1, 0), (0, 0, 2, 1, 0), (0, 0, -1, 1, 0), (0, 0, 0, 0, 0), (0, 0, 0, 149, 0), (0, 147, 0, 2, 0),
+        (big, big, big, big, 0), (0, big, 0, 1, 0), (0, 1, 0, big, 0), (-big, -big, -big, -big, 0), (0, 0, 0, -big, 0),
+    ]:
+        assert ok(item, run, slot, parts, 12, 148) == good, (item, run, slot, parts)
 
 
 # --------------------------------------------------------------------- GPU

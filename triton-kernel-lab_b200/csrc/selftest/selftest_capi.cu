@@ -8,6 +8,7 @@
 #include "../../../include/tklab_attn.h"
 #include "../attn_fwd_split_plan.h"
 #include "../sm100_primitives.cuh"
+#include "../tree_attn_plan.h"
 #include "tklab_selftest.h"
 #include "tklab_selftest_impl.h"
 
@@ -135,6 +136,10 @@ int tk_selftest_fwd_split_plan(int64_t bh, int64_t seq, int64_t head_dim, int ca
 
 void tk_selftest_fwd_split_decode(int u, int bh, int n_ctiles, int causal, int kt, int split_l, int* out) {
   if (out != nullptr) tk::fwd_split_decode(u, bh, n_ctiles, causal, kt, split_l, out);
+}
+
+int tk_selftest_tree_cut_ok(int item, int run, int slot, int parts, int items, int runs) {
+  return tk::tree_cut_ok({item, run, slot, parts}, items, runs) ? 1 : 0;
 }
 
 int tk_selftest_status(int* status_out, void* stream) {

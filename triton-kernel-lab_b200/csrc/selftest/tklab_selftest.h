@@ -44,6 +44,11 @@ TKS_API int tk_selftest_fwd_split_plan(int64_t bh, int64_t seq, int64_t head_dim
  * group, chunk.  Host code only. */
 TKS_API void tk_selftest_fwd_split_decode(int u, int bh, int n_ctiles, int causal, int kt, int split_l, int* out);
 
+/* Whether the tree attention's joining kernel takes a plan entry (item, run,
+ * slot, parts) for a cut item among `items` items and `runs` runs
+ * (csrc/tree_attn_plan.h).  Host code only. */
+TKS_API int tk_selftest_tree_cut_ok(int item, int run, int slot, int parts, int items, int runs);
+
 /* Synchronise `stream`, then read and clear this library's device status
  * word (the first error a probe kernel recorded). */
 TKS_API int tk_selftest_status(int* status_out, void* stream);

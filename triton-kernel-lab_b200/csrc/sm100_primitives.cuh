@@ -124,6 +124,16 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, CtaCon
   }
 }
 
+// Wait for phase `parity` of `bar` in a CTA that has given up: for a copy or a
+// product that is under way, at most kDrainNs, whatever the abort flag says.
+constexpr uint64_t kDrainNs = 100000000ull;
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  const uint64_t start = global_timer_ns();
+  while (!mbar_try_wait(addr, parity) && global_timer_ns() - start < kDrainNs) {
+  }
+}
+
 // ---------------------------------------------------------------------------
 // TMA (cp.async.bulk.tensor), no multicast anywhere.
 // ---------------------------------------------------------------------------

@@ -68,6 +68,7 @@
 #include "attn_launch.h"
 #include "pdl_launch.h"
 #include "sm100_primitives.cuh"
+#include "tree_attn_plan.h"
 
 namespace tk {
 namespace {
@@ -102,8 +103,8 @@ struct TreeCfg {
   static constexpr int kJoinCols = 64;  // columns of O joined at a time (every copy, fp32)
   static constexpr int kBarOff = kJoinOff + (kRep > 1 ? kTileRows * kJoinCols * 4 : 0);
   // q_full[Q], q_empty[Q], k_full[S], k_empty[S], v_full[S], v_ok[S], v_empty[S], s_full[2], p_ready[2], o_final[2],
-  // o_empty[2], l_ready[2], pv_done
-  static constexpr int kNumBars = 2 * kQBufs + 2 * kStages + 3 * kVStages + 11;
+  // o_empty[2], l_ready[2], pv_done, drained
+  static constexpr int kNumBars = 2 * kQBufs + 2 * kStages + 3 * kVStages + 12;
   static constexpr int kCtlOff = kBarOff + kNumBars * 8;
   static constexpr int kMlOff = (kCtlOff + 16 + 32 + 64 + 7) / 8 * 8;  // after control, first segment, scan
   // m and l of a segment's rows, two buffers.
@@ -188,11 +189,9 @@ struct TreeWalk {
 };
 
 // The start of the workspace, for the joining kernel: an entry per item or, if
-// there are fewer runs, per run, written by the CTA that begins the item: the
-// cut item (b Hkv + h, -1: none), the run of its first part, that part's slot
-// and the number of parts.
+// there are fewer runs, per run, written by the CTA that begins the item.
 struct TreePlan {
-  int4* cut;
+  TreeCut* cut;
   int by_item;
   int whole;  // a CTA per item, grid (groups, items): nothing else of the plan or the workspace is used
 };
@@ -629,11 +628,13 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
   uint64_t* o_empty = o_final + 2;          // [2]: O buffer read by the epilogue
   uint64_t* l_ready = o_empty + 2;          // [2]: m and l of O buffer's segment written
   uint64_t* pv_done = l_ready + 2;          // with two S buffers: P V of every tile
+  uint64_t* drained = pv_done + 1;          // after a wait that gave up: every product
   CtaControl* ctl = reinterpret_cast<CtaControl*>(smem + C::kCtlOff);
   // Values that are not finite were taken out of a tree tile of this CTA.  Warp 3
   // sets it before v_ok of the tile, which the softmax warps wait for.
   volatile int* patched = reinterpret_cast<int*>(smem + C::kCtlOff + sizeof(CtaControl));
   int* first = reinterpret_cast<int*>(smem + C::kCtlOff + 16);  // this CTA's run: b, h, u, length; the runs' length
+  int* loads = first + 5;  // [3]: tiles of K (warp 0) and V (warp 2) and segments' Q (warp 3) that were asked for
   int* scan = first + 8;                                         // [warps]
 
   // Loads of the query rows of a segment (kT tiles of 128 rows, or kRep copies
@@ -794,31 +795,33 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
             load_tile(seg, j, is_k, st);
           }
         }
+        loads[warp >> 1] = max(g, is_k ? early : 0u);
       }
     } else if (warp == 3) {
       // ---------------- Q, the tails of V, and the joining kernel's entries ----------------
-      int4 mine = make_int4(-1, 0, 0, 0);
+      TreeCut mine{-1, 0, 0, 0};
       uint32_t g = 0;
+      int asked = 0;
       bool ok = true;
-      for (int it = 0; ok && walk.next(shape, seg); ++it) {
-        const int qb = it % C::kQBufs;
-        if (it >= C::kQBufs &&
-            !(ok = warp_wait(&q_empty[qb], ((it / C::kQBufs) & 1) ^ 1, ctl, timeout_ns, status, 1)))
-          break;
-        if (lane == 0) {
-          if (!by_warp || it > 0) load_q(seg, qb);
-          if (!whole_item && group == 0 && seg.j0 == 0) {
-            const bool cut = seg.j1 < seg.n_all;
-            const int item = seg.b * shape.Hkv + seg.h;
-            const int4 e = cut ? make_int4(item, blockIdx.y, it > 0 ? 1 : 0,
-                                           1 + (seg.n_all - seg.j1 + first[4] - 1) / first[4])
-                               : make_int4(-1, 0, 0, 0);
-            if (plan.by_item)
-              plan.cut[item] = e;
-            else if (cut)
-              mine = e;
-          }
+      // (Every segment, failed or not: an entry is for the joining kernel to read.)
+      for (int it = 0; walk.next(shape, seg); ++it) {
+        if (lane == 0 && !whole_item && group == 0 && seg.j0 == 0) {
+          const bool cut = seg.j1 < seg.n_all;
+          const int item = seg.b * shape.Hkv + seg.h;
+          const TreeCut e{cut ? item : -1, static_cast<int>(blockIdx.y), it > 0 ? 1 : 0,
+                          1 + (seg.n_all - seg.j1 + first[4] - 1) / first[4]};
+          if (plan.by_item)
+            plan.cut[item] = e;
+          else if (cut)
+            mine = e;
         }
+        const int qb = it % C::kQBufs;
+        if (ok && it >= C::kQBufs) ok = warp_wait(&q_empty[qb], ((it / C::kQBufs) & 1) ^ 1, ctl, timeout_ns, status, 1);
+        if (!ok) continue;
+        if (!by_warp || it > 0) {
+          if (lane == 0) load_q(seg, qb);
+        }
+        asked = it + 1;
         const int size = tree_size(shape, seg.b);
         for (int j = seg.j0; j < seg.j1; ++j, ++g) {
           const int st = g % C::kVStages;
@@ -843,6 +846,7 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
         }
       }
       if (lane == 0 && !whole_item && group == 0 && !plan.by_item) plan.cut[blockIdx.y] = mine;
+      if (lane == 0) loads[2] = asked;
     } else if (warp == 1) {
       // ---------------- MMA issuer ----------------
       const bool leader = elect_one();
@@ -1081,6 +1085,23 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (ctl->abort != 0) {
+    // A wait gave up: copies and products may be under way, which have to end
+    // before the CTA's shared and tensor memory are another's.
+    if (warp == 1) {
+      if (elect_one()) umma_commit(drained);
+      __syncwarp();
+      mbar_drain(drained, 0);
+      auto drain = [&](uint64_t* full, int depth, int n) {
+#pragma unroll 1
+        for (int i = max(n - depth, 0); i < n; ++i) mbar_drain(&full[i % depth], (i / depth) & 1);
+      };
+      drain(k_full, C::kStages, loads[0]);
+      drain(v_full, C::kVStages, loads[1]);
+      drain(q_full, C::kQBufs, loads[2]);
+    }
+    __syncthreads();
+  }
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -1099,13 +1120,13 @@ template <int D, bool kBf16, int kShare>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     tree_attn_combine_kernel(const __grid_constant__ TreeShape shape, uint16_t* __restrict__ out,
                              float* __restrict__ lse, TreePlan plan, const float* __restrict__ part_ml,
-                             const float* __restrict__ part_o, int groups, int group_rows) {
+                             const float* __restrict__ part_o, int groups, int runs, int group_rows) {
   constexpr int kVec = D / 32;  // float4 of a part's four rows a lane
   constexpr int kBatch = 4;
   pdl_launch_dependents();
   pdl_wait_prerequisites();
-  const int4 cut = plan.cut[blockIdx.y];
-  if (cut.x < 0) return;
+  const TreeCut cut = plan.cut[blockIdx.y];
+  if (!tree_cut_ok(cut, shape.B * shape.Hkv, runs)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int share = warp % kShare;
   const int row0 = (blockIdx.x * (kJoinWarps / kShare) + warp / kShare) * 4;
@@ -1116,7 +1137,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   float4 acc[kVec];
 #pragma unroll
   for (int e = 0; e < kVec; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int p = share; p < cut.w; p += kShare * kBatch) {
+  for (int p = share; p < cut.parts; p += kShare * kBatch) {
     float2 ml[kBatch];
     float4 v[kBatch][kVec];
 #pragma unroll
@@ -1125,8 +1146,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
       ml[i] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) v[i][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (pi < cut.w && row_ok) {
-        const long long slot = (static_cast<long long>(cut.y + pi) * groups + group) * 2 + (pi == 0 ? cut.z : 0);
+      if (pi < cut.parts && row_ok) {
+        const long long slot = (static_cast<long long>(cut.run + pi) * groups + group) * 2 + (pi == 0 ? cut.slot : 0);
         const long long prow0 = slot * group_rows + row0 % group_rows;
         ml[i] = *reinterpret_cast<const float2*>(part_ml + (prow0 + (row - row0)) * 2);
         const float4* src = reinterpret_cast<const float4*>(part_o + prow0 * D) + lane;
@@ -1183,7 +1204,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
     }
   }
   if (!row_ok) return;
-  const long long row_g = static_cast<long long>(cut.x) * shape.R + row;
+  const long long row_g = static_cast<long long>(cut.item) * shape.R + row;
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // of a NaN: NaN
 #pragma unroll
   for (int e = 0; e < kVec; ++e) {
@@ -1241,7 +1262,7 @@ TreeGrid tree_grid(int64_t B, int64_t Hkv, int64_t G, int64_t T, int64_t L, int6
   t.runs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / t.groups, items * (item_tiles + kItemCost))));
   const size_t rows = static_cast<size_t>(t.groups) * t.runs * 2 * group_rows;
   t.cuts = static_cast<int>(std::min<int64_t>(items, t.runs));
-  t.plan_bytes = (static_cast<size_t>(t.cuts) * sizeof(int4) + 255) / 256 * 256;
+  t.plan_bytes = (static_cast<size_t>(t.cuts) * sizeof(TreeCut) + 255) / 256 * 256;
   t.ml_bytes = rows * 8;
   t.o_bytes = rows * static_cast<size_t>(width) * 4;
   return t;
@@ -1253,7 +1274,7 @@ int launch_tree_combine(const TreeAttnArgs& a, const TreeGrid& t, const TreeShap
   const int64_t per_block = kJoinWarps / kShare * 4;
   const dim3 grid(static_cast<unsigned>((a.G * a.T + per_block - 1) / per_block), static_cast<unsigned>(t.cuts));
   return launch_pdl(tree_attn_combine_kernel<D, kBf16, kShare>, grid, dim3(32 * kJoinWarps), 0, a.stream, 1, shape,
-                    static_cast<uint16_t*>(a.o), a.lse, plan, part_ml, part_o, t.groups, group_rows);
+                    static_cast<uint16_t*>(a.o), a.lse, plan, part_ml, part_o, t.groups, t.runs, group_rows);
 }
 
 template <int D, int kT, int kRep, bool kBf16>
@@ -1267,7 +1288,7 @@ int launch_tree_t(const TreeAttnArgs& a, const TreeGrid& t) {
                         static_cast<int>(a.Hkv), static_cast<int>(a.T), static_cast<int>(a.L),
                         static_cast<int>(a.G * a.T), static_cast<int>(a.D)};
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
-  const TreePlan plan{reinterpret_cast<int4*>(ws), a.B * a.Hkv <= t.runs ? 1 : 0, t.whole ? 1 : 0};
+  const TreePlan plan{reinterpret_cast<TreeCut*>(ws), a.B * a.Hkv <= t.runs ? 1 : 0, t.whole ? 1 : 0};
   float* part_ml = reinterpret_cast<float*>(ws + t.plan_bytes);
   float* part_o = reinterpret_cast<float*>(ws + t.plan_bytes + t.ml_bytes);
   const dim3 grid(static_cast<unsigned>(t.groups), static_cast<unsigned>(t.whole ? a.B * a.Hkv : t.runs));
