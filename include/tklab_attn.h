@@ -247,7 +247,8 @@ TK_API int tk_rotary(const void* q, const void* k, void* q_out, void* k_out, con
  *   k, v            (batch, kv_heads, seq_kv, head_dim) cache
  *   k_tree, v_tree  (batch, kv_heads, nodes, head_dim) the tree's own rows
  *   strides         12 element strides: k, v, k_tree, v_tree x (batch, head,
- *                   row), multiples of 8; columns contiguous
+ *                   row), multiples of 8, not 0 where there is more than one;
+ *                   columns contiguous
  *   kv_lens         (batch) int32 valid cache rows, clamped to [0, seq_kv]
  *   parents         (batch, nodes) int32 with a stride of parent_stride
  *                   (nodes, or 0 for one tree shared by all), parents[t] < t,

@@ -475,3 +475,31 @@ def test_many_small_weights_beside_a_large_one(group: int, nodes: int, dtype: to
     assert bool((err <= bound).all()), float((err / bound).max())
     assert torch.allclose(lse.double().cpu(), ref_lse.expand(batch, -1, -1), atol=2e-4)
     check_device_status()
+
+
+@pytest.mark.parametrize("place", [1, 4, 7, 10, 2, 11])
+def test_library_refuses_strides_of_zero(place: int) -> None:
+    """Rows or heads that are one in memory: no tensor map describes them."""
+    strides = [64] * 12
+    strides[place] = 0
+    args = {"q": 0x1000, "k": 0x1000, "v": 0x1000, "k_tree": 0x1000, "v_tree": 0x1000, "strides": (ctypes.c_int64 * 12)(*strides),
+            "kv_lens": 0x1000, "parents": None, "parent_stride": 0, "tree_sizes": None, "o": 0x1000, "lse": None, "workspace": None,
+            "workspace_bytes": 0, "batch": 1, "q_heads": 4, "kv_heads": 2, "nodes": 3, "seq_kv": 16, "head_dim": 64, "dtype": 1,
+            "scale": 0.125, "stream": None}
+    assert _native.load().tk_tree_attn(*args.values()) == 1
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("across", [(0,), (1,), (2,), (0, 1), (0, 1, 2)])
+def test_trees_that_repeat_in_memory(across: tuple[int, ...]) -> None:
+    g = on_gpu(problem(3, 8, 4, 5, 64, 70, [70, 1, 40], torch.bfloat16, seed=13))
+    one = {}
+    for name in ("k_tree", "v_tree"):
+        part = g[name]
+        for axis in across:
+            part = part.narrow(axis, 0, 1)
+        one[name] = part.expand(3, 4, 5, 64)
+    ref = tree_attention(**{**g, **{n: t.contiguous() for n, t in one.items()}})
+    assert torch.equal(tree_attention(**{**g, **one}), ref)
+    check_device_status()

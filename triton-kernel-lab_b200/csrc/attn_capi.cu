@@ -500,6 +500,10 @@ int tk_tree_attn(const void* q, const void* k, const void* v, const void* k_tree
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return tk::kErrMisaligned;
   for (int i = 0; i < 12; ++i)
     if (strides[i] < 0 || strides[i] % 8 != 0) return tk::kErrMisaligned;
+  // The tensor maps describe distinct rows: a stride of 0 is not one of theirs.
+  const int64_t sizes[3][2] = {{batch, batch}, {kv_heads, kv_heads}, {seq_kv, nodes}};
+  for (int i = 0; i < 12; ++i)
+    if (strides[i] == 0 && sizes[i % 3][i / 6] > 1) return tk::kErrInvalidArgument;
   tk::TreeAttnArgs a{};
   if (int rc = status_ptr(&a.status)) return rc;
   a.sms = sm_count();

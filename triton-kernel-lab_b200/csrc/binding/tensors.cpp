@@ -50,9 +50,9 @@ bool row_strides(const Tensor& t, int64_t* out) {
   return true;
 }
 
-// A cache: no two rows in one place.
+// No two rows in one place, as a cache and what a tensor map describes need.
 template <int N>
-bool cache_strides(const Tensor& t, int64_t* out) {
+bool distinct_strides(const Tensor& t, int64_t* out) {
   if (!row_strides<N>(t, out)) return false;
   for (int i = 0; i < N; ++i)
     if (out[i] == 0 && t.size(i) > 1) return false;
@@ -248,8 +248,8 @@ PyObject* py_tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int64_t strides[12], parent_stride;
   for (const Tensor& t : {k, v, kt, vt})
     if (!like(t, q.scalar_type(), q)) Py_RETURN_NONE;
-  if (!q.is_contiguous() || !aligned16(q) || !cache_strides<3>(k, strides) || !cache_strides<3>(v, strides + 3) ||
-      !row_strides<3>(kt, strides + 6) || !row_strides<3>(vt, strides + 9) || !ints(lens, q, {batch}) ||
+  if (!q.is_contiguous() || !aligned16(q) || !distinct_strides<3>(k, strides) || !distinct_strides<3>(v, strides + 3) ||
+      !distinct_strides<3>(kt, strides + 6) || !distinct_strides<3>(vt, strides + 9) || !ints(lens, q, {batch}) ||
       !parents_ok(parents, q, batch, nodes, &parent_stride) || (sizes.defined() && !ints(sizes, q, {batch})))
     Py_RETURN_NONE;
   double scale = 1.0 / std::sqrt(static_cast<double>(dim));
@@ -336,7 +336,7 @@ PyObject* py_commit_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor& t = *all[i];
     int64_t* s = strides + 4 * i;
     if (!like(t, k.scalar_type(), k)) Py_RETURN_NONE;
-    const bool ok = i < 2 ? (first == 1 ? cache_strides<4>(t, s) : cache_strides<3>(t, s + 1))
+    const bool ok = i < 2 ? (first == 1 ? distinct_strides<4>(t, s) : distinct_strides<3>(t, s + 1))
                           : (first == 1 ? row_strides<4>(t, s) : row_strides<3>(t, s + 1));
     if (!ok) Py_RETURN_NONE;
   }

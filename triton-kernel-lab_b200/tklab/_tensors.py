@@ -61,14 +61,24 @@ def rows_in_place(x: torch.Tensor) -> bool:
     )
 
 
+def rows_repeat(x: torch.Tensor) -> bool:
+    """Whether some of ``x``'s rows are one in memory (an expanded tensor)."""
+    return any(s == 0 and n > 1 for s, n in zip(x.stride()[:-1], x.shape))
+
+
 def dense(x: torch.Tensor) -> torch.Tensor:
     """``x`` itself if the kernels can read it, else a contiguous copy (differentiable)."""
     return x if rows_in_place(x) else x.clone(memory_format=torch.contiguous_format)
 
 
+def distinct(x: torch.Tensor) -> torch.Tensor:
+    """:func:`dense` for what a tensor map describes: repeated rows are copied, too."""
+    return dense(x.contiguous() if rows_repeat(x) else x)
+
+
 def require_cache(x: torch.Tensor, name: str) -> None:
     """Refuse a cache that would have to be copied (it is written in place, or too large) or repeats rows."""
-    if not rows_in_place(x) or any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
+    if not rows_in_place(x) or rows_repeat(x):
         raise ValueError(f"{name} needs contiguous, 16-byte aligned rows at distinct strides that are multiples of 8")
 
 

@@ -16,7 +16,7 @@ import math
 
 import torch
 
-from tklab._tensors import binding, contiguous, dense, require_cache
+from tklab._tensors import binding, contiguous, dense, distinct, require_cache
 from tklab.kernels.flash_attention import _NATIVE_DTYPE, _after_launch
 
 MAX_TREE_NODES = 256
@@ -73,7 +73,7 @@ def _prepare(q, k_cache, v_cache, k_tree, v_tree, kv_lens, parents, tree_sizes, 
     require_cache(k_cache, "the K cache")
     require_cache(v_cache, "the V cache")
     return (
-        dense(q.contiguous()), k_cache, v_cache, dense(k_tree), dense(v_tree), kv_lens.contiguous(), contiguous(parents),
+        dense(q.contiguous()), k_cache, v_cache, distinct(k_tree), distinct(v_tree), kv_lens.contiguous(), contiguous(parents),
         contiguous(tree_sizes), scale,
     )
 
