@@ -503,3 +503,25 @@ def test_trees_that_repeat_in_memory(across: tuple[int, ...]) -> None:
     ref = tree_attention(**{**g, **{n: t.contiguous() for n, t in one.items()}})
     assert torch.equal(tree_attention(**{**g, **one}), ref)
     check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("which", ["q", "k_cache", "v_cache", "k_tree", "v_tree"])
+def test_a_gradient_through_it_is_an_error(which: str) -> None:
+    """No derivative: a loss that depends on it says so in its backward pass, it does not lose a term."""
+    g = on_gpu(problem(2, 4, 2, 5, 64, 40, [40, 7], torch.bfloat16, seed=14))
+    ref, ref_lse = tree_attention(**g, return_lse=True)
+    g[which].requires_grad_(True)
+    o, lse = tree_attention(**g, return_lse=True)
+    assert torch.equal(o, ref) and torch.equal(lse, ref_lse)
+    for out in (o, lse, tree_attention(**g)):
+        with pytest.raises(RuntimeError, match="no derivative"):
+            out.float().sum().backward()
+    assert g[which].grad is None
+    with torch.no_grad():
+        o = tree_attention(**g)
+    assert not o.requires_grad and torch.equal(o, ref)
+    o = tree_attention(**{**g, which: g[which].detach()})
+    assert not o.requires_grad and torch.equal(o, ref)
+    check_device_status()

@@ -15,6 +15,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
@@ -229,6 +230,25 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The history of a result without a derivative: one that asks for it learns of it.
+struct NoDerivative : torch::autograd::Node {
+  torch::autograd::variable_list apply(torch::autograd::variable_list&&) override {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "tree_attention has no derivative (it serves inference): call it under torch.no_grad() "
+                                       "or on detached tensors");
+  }
+};
+
+void mark_no_derivative(std::initializer_list<Tensor> inputs, std::initializer_list<Tensor> outputs) {
+  if (!at::GradMode::is_enabled()) return;
+  bool needed = false;
+  for (const Tensor& t : inputs) needed = needed || t.requires_grad();
+  if (!needed) return;
+  std::shared_ptr<torch::autograd::Node> node(new NoDerivative(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(torch::autograd::variable_list(inputs)));
+  for (const Tensor& t : outputs)
+    if (t.defined()) torch::autograd::set_history(t, node);
+}
+
 PyObject* py_tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arity(n, 10)) return nullptr;
@@ -270,6 +290,7 @@ PyObject* py_tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
                      bytes > 0 ? workspace.data_ptr() : nullptr, bytes, batch, q_heads, kv_heads, nodes, rows, dim,
                      attn_dtype(q), static_cast<float>(scale), on.handle()),
         "tk_tree_attn");
+  mark_no_derivative({q, k, v, kt, vt}, {out, lse});
   return return_lse ? tuple_of({out, lse}) : THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }

@@ -105,6 +105,9 @@ def tree_attention(
         tree_sizes: (batch,) int32, nodes in use; the rest get 0 and an lse of -inf.
         scale: default ``1 / sqrt(head_dim)``.
 
+    It serves inference: there is no derivative, and a backward pass that
+    reaches it raises.
+
     Returns ``o`` shaped like ``q`` (and the base-2 log-sum-exp, scale
     included, (batch, q_heads, nodes) fp32 when ``return_lse``).
     """
