@@ -259,3 +259,21 @@ def test_gradient_of_the_gradient_and_without_positions() -> None:
     (g,) = torch.autograd.grad(rotary(q, k.detach(), cos, sin)[0], q, dq.detach())
     assert torch.equal(g, gq)
     check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("order", ["bhsd", "bshd"])
+def test_a_tangent_through_it_is_an_error(which: int, order: str) -> None:
+    """Forward-mode differentiation is refused, with requires_grad or without; a tangent is not lost."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    cos, sin = rotary_tables(5, 64, device="cuda")
+    x = [make((1, 2, 5, 64), torch.float16, gen, order) for _ in range(2)]
+    with torch.autograd.forward_ad.dual_level():
+        x[which] = torch.autograd.forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            rotary(*x, cos, sin)
+        x[which].requires_grad_(True)
+        with pytest.raises(RuntimeError):
+            rotary(*x, cos, sin)

@@ -321,3 +321,14 @@ def test_commit_into_a_full_cache_and_bad_paths() -> None:
         check_device_status()
     assert torch.equal(g[0][:, :, :, 1:], before[:, :, :, 1:])
     check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("which", [0, 3])
+def test_commit_of_a_tangent_is_an_error(which: int) -> None:
+    g = [t.cuda() for t in commit_problem(1, 2, 2, 5, 20, 64, torch.bfloat16, seed=4)]
+    with torch.autograd.forward_ad.dual_level():
+        g[which] = torch.autograd.forward_ad.make_dual(g[which], torch.ones_like(g[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            commit_draft(*g)

@@ -525,3 +525,14 @@ def test_a_gradient_through_it_is_an_error(which: str) -> None:
     o = tree_attention(**{**g, which: g[which].detach()})
     assert not o.requires_grad and torch.equal(o, ref)
     check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("which", ["q", "v_cache", "k_tree"])
+def test_a_tangent_through_it_is_an_error(which: str) -> None:
+    g = on_gpu(problem(2, 4, 2, 5, 64, 40, [40, 7], torch.bfloat16, seed=14))
+    with torch.autograd.forward_ad.dual_level():
+        g[which] = torch.autograd.forward_ad.make_dual(g[which], torch.ones_like(g[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            tree_attention(**g)

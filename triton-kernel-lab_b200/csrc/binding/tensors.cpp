@@ -189,6 +189,12 @@ bool tensor_arg(PyObject* o, Tensor* t, bool optional = false) {
   return true;
 }
 
+// The operators know no forward mode: a tangent that would be lost is an error.
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
   PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
   if (out == nullptr) return nullptr;
@@ -221,6 +227,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
   r.interleaved = PyObject_IsTrue(args[5]) == 1;
   if (!rotary_ok(q, k, r)) Py_RETURN_NONE;
+  refuse_tangents("rotary", {&q, &k});
   if (at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
     const auto out = RotaryFunction::apply(q, given(k), r.cos.detach(), r.sin.detach(), given(r.positions), r.interleaved, false);
     return tuple_of({out[0], k.defined() ? out[1] : Tensor()});
@@ -279,6 +286,7 @@ PyObject* py_tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!std::isfinite(scale) || scale <= 0.0) Py_RETURN_NONE;
   }
   const bool return_lse = PyObject_IsTrue(args[9]) == 1;
+  refuse_tangents("tree_attention", {&q, &k, &v, &kt, &vt});
   const Launch on(q);
   const size_t bytes = tk_tree_attn_workspace_bytes(batch, q_heads, kv_heads, nodes, rows, dim);
   Tensor out = fresh(q.sizes(), q.scalar_type(), q), lse, workspace;
@@ -362,6 +370,7 @@ PyObject* py_commit_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!ok) Py_RETURN_NONE;
   }
   if (!ints(path, k, {batch, nodes}) || !ints(path_lens, k, {batch}) || !ints(lens, k, {batch})) Py_RETURN_NONE;
+  refuse_tangents("commit_draft", {&k, &v, &kt, &vt});
   const Launch on(k);
   Tensor out = fresh({batch}, at::kInt, k);
   check(tk_commit_draft(k.data_ptr(), v.data_ptr(), kt.const_data_ptr(), vt.const_data_ptr(), strides,

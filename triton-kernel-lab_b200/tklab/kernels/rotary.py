@@ -160,7 +160,7 @@ def rotary(
     position outside the tables leaves its rows as they are and is reported
     by :func:`tklab.kernels.flash_attention.check_device_status`.  Returns
     contiguous (batch, heads, seq, head_dim) tensors; differentiable in ``q``
-    and ``k``.
+    and ``k`` (backward passes of any order; forward mode is refused).
     """
     if layout not in ROTARY_LAYOUTS:
         raise ValueError(f"rotary layout must be one of {ROTARY_LAYOUTS}")
