@@ -332,3 +332,28 @@ def test_commit_of_a_tangent_is_an_error(which: int) -> None:
         g[which] = torch.autograd.forward_ad.make_dual(g[which], torch.ones_like(g[which]))
         with pytest.raises(RuntimeError, match="forward-mode"):
             commit_draft(*g)
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("which", [0, 1])
+def test_commit_is_a_change_in_place(which: int) -> None:
+    """What autograd saved of a cache before is known to be stale after, a view of one layer included."""
+    for layers in (False, True):
+        g = [t.cuda() for t in commit_problem(2, 2, 2, 5, 20, 64, torch.bfloat16, seed=5)]
+        x = torch.ones((), device="cuda", requires_grad=True)
+        loss = (x * g[which].float().mul_(1.0)).sum() + (x.bfloat16() * g[which]).sum()
+        before = g[which]._version
+        if layers:
+            commit_draft(*g)
+        else:
+            commit_draft(*(t[1] for t in g[:4]), *g[4:])
+        assert g[which]._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        g = [t.cuda() for t in commit_problem(1, 2, 2, 5, 20, 64, torch.bfloat16, seed=5)]
+        want = commit_reference(*(t.cpu() for t in g))
+        commit_draft(*g)
+        assert torch.equal(g[0].cpu(), want[0]) and torch.equal(g[1].cpu(), want[1])
+    check_device_status()

@@ -377,6 +377,9 @@ PyObject* py_commit_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
                         path.const_data_ptr<int>(), path_lens.const_data_ptr<int>(), lens.const_data_ptr<int>(),
                         out.data_ptr<int>(), layers, batch, heads, nodes, rows, dim, on.handle()),
         "tk_commit_draft");
+  // Written in place: what autograd has saved of the caches is stale.
+  for (const Tensor* t : {&k, &v})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
