@@ -357,3 +357,25 @@ def test_commit_is_a_change_in_place(which: int) -> None:
         commit_draft(*g)
         assert torch.equal(g[0].cpu(), want[0]) and torch.equal(g[1].cpu(), want[1])
     check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize(
+    ("path_len", "kv_len", "rows", "start", "match"),
+    [(7, 3, 6, 3, "invalid argument"), (-1, 3, 0, 3, "invalid argument"), (2, -4, 2, 0, "invalid argument"),
+     (0, 21, 0, 20, "invalid argument"), (2, 21, 0, 20, "exceeds"), (6, 14, 6, 14, None), (0, 20, 0, 20, None)],
+)
+def test_commit_reports_lengths_that_it_clamps(path_len: int, kv_len: int, rows: int, start: int, match: str | None) -> None:
+    args = [t.cuda() for t in commit_problem(2, 2, 3, 6, 20, 64, torch.float16, seed=8)]
+    args[4] = torch.arange(6, dtype=torch.int32, device="cuda").expand(2, 6).contiguous()
+    args[5], args[6] = (torch.tensor([n, 1], dtype=torch.int32, device="cuda") for n in (path_len, kv_len))
+    want = args[0].clone()
+    want[:, 0, :, start : start + rows] = args[2][:, 0, :, :rows]
+    want[:, 1, :, 1] = args[2][:, 1, :, 0]
+    assert commit_draft(*args).tolist() == [start + rows, 2]
+    assert torch.equal(args[0], want)
+    if match is not None:
+        with pytest.raises(RuntimeError, match=match):
+            check_device_status()
+    check_device_status()

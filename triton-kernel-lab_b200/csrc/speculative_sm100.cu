@@ -395,12 +395,14 @@ __global__ void __launch_bounds__(kCommitThreads) commit_kernel(const __grid_con
   pdl_wait_prerequisites();
   const int64_t b = blockIdx.x % a.B, layer = blockIdx.x / a.B;
   const int h0 = blockIdx.y * kCommitHeads, heads = min(kCommitHeads, static_cast<int>(a.H) - h0);
-  const int n = min(max(a.path_lens[b], 0), static_cast<int>(a.T));
-  const int start = min(max(a.kv_lens[b], 0), static_cast<int>(a.L));
+  const int path_len = a.path_lens[b], kv_len = a.kv_lens[b];
+  const int n = min(max(path_len, 0), static_cast<int>(a.T));
+  const int start = min(max(kv_len, 0), static_cast<int>(a.L));
   const int fit = min(n, static_cast<int>(a.L) - start);
   if (h0 == 0 && layer == 0 && threadIdx.x == 0) {
     a.new_lens[b] = start + fit;
     if (fit < n) atomicCAS(a.status, kOk, kErrTooLarge);
+    if (n != path_len || start != kv_len) atomicCAS(a.status, kOk, kErrInvalidArgument);
   }
   const int lane_row = threadIdx.x / chunks, c = threadIdx.x % chunks * 8;
   if (lane_row >= rows) return;

@@ -174,8 +174,9 @@ def commit_draft(
     cache row ``kv_lens[b] + i``.  Caches (batch, kv_heads, seq_kv, head_dim) with
     trees (batch, kv_heads, nodes, head_dim), or both with a leading layers
     dimension: all layers are then written in one launch.  Rows are copied as
-    data, no gradient goes through the cache.  Rows that the cache
-    has no room for are left out, the returned length stops at ``seq_kv`` and
+    data, no gradient goes through the cache.  Rows that the cache has no room
+    for are left out and the returned length stops at ``seq_kv``; ``path_lens``
+    outside 0..nodes and ``kv_lens`` outside 0..seq_kv are clamped; in either case
     :func:`tklab.kernels.flash_attention.check_device_status` raises.
     """
     args = (k_cache, v_cache, k_tree, v_tree, path, path_lens, kv_lens)
