@@ -311,7 +311,8 @@ TK_API int tk_verify_draft(const void* target, const int64_t* target_strides, co
  * at seq_kv and TK_ERR_TOO_LARGE goes to the device status word; a path entry
  * outside [0, nodes) is skipped, and path_lens outside [0, nodes] and kv_lens
  * outside [0, seq_kv] are clamped, with TK_ERR_INVALID_ARGUMENT.  new_lens may
- * not be kv_lens. */
+ * not be kv_lens, and k_tree and v_tree may not overlap the rows written: the
+ * kernel copies rows in any order. */
 TK_API int tk_commit_draft(void* k, void* v, const void* k_tree, const void* v_tree, const int64_t* strides,
                            const int32_t* path, const int32_t* path_lens, const int32_t* kv_lens, int32_t* new_lens,
                            int64_t layers, int64_t batch, int64_t kv_heads, int64_t nodes, int64_t seq_kv,

@@ -4,12 +4,14 @@ from __future__ import annotations
 
 import ctypes
 import math
+import random
 
 import pytest
 import torch
 
 from oracle.speculative_oracle import commit_reference, verify_reference
 from tklab import _native
+from tklab._tensors import binding
 from tklab.kernels.flash_attention import check_device_status
 from tklab.kernels.speculative import commit_draft, verify_draft
 
@@ -126,6 +128,31 @@ def test_library_commit_refuses_before_launch(kwargs: dict, status: int) -> None
             "kv_heads": 1, "nodes": 3, "seq_kv": 8, "head_dim": 16, "stream": None}
     args.update(kwargs)
     assert _native.load().tk_commit_draft(*args.values()) == status
+
+
+def test_overlap_of_trees_and_caches_is_found() -> None:
+    """Against the sets of elements: views of one buffer in every order of dimensions, whole and in part, near and far."""
+    gen = random.Random(1)
+    apart = 0
+    for _ in range(2000):
+        sizes = [gen.randint(1, 4) for _ in range(3)] + [gen.randint(4, 9), 8]
+        order = gen.sample(range(4), 4) + [4]
+        buffer = torch.arange(math.prod(sizes), dtype=torch.int16).view([sizes[i] for i in order])
+        whole = buffer.permute([order.index(i) for i in range(5)])
+        views = []
+        for _ in range(2):
+            view = whole
+            for axis in range(5):
+                if gen.random() < (0.8 if axis == 3 else 0.3):
+                    start = gen.randrange(sizes[axis])
+                    view = view.narrow(axis, start, gen.randint(1, sizes[axis] - start))
+            views.append(view)
+        common = not set(views[0].flatten().tolist()).isdisjoint(views[1].flatten().tolist())
+        assert binding.may_overlap(*views) == common
+        apart += not common
+    assert 200 < apart < 1800
+    other = torch.arange(64, dtype=torch.int16)
+    assert not binding.may_overlap(other[:32], other[32:].clone()) and binding.may_overlap(other[::2], other[1::3])  # not known
 
 
 # ------------------------------------------------------------ verification
@@ -378,4 +405,57 @@ def test_commit_reports_lengths_that_it_clamps(path_len: int, kv_len: int, rows:
     if match is not None:
         with pytest.raises(RuntimeError, match=match):
             check_device_status()
+    check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+@pytest.mark.parametrize("layers", [1, 3])
+def test_commit_of_drafts_kept_in_the_cache(layers: int) -> None:
+    """Trees that are rows of the caches, before, behind and among those written: copied as they were before the call."""
+    for which in range(4):
+        args = [t.cuda() for t in commit_problem(layers, 4, 3, 9, 40, 64, torch.bfloat16, seed=9)]
+        args[4] = torch.tensor([[0, 2, 3, 5, 8, -1, -1, -1, -1]] * 4, dtype=torch.int32, device="cuda")
+        args[5] = torch.tensor([5, 4, 5, 1], dtype=torch.int32, device="cuda")
+        args[6] = torch.tensor([10, 12, 8, 15], dtype=torch.int32, device="cuda")
+        if which in (0, 2):
+            args[2] = args[0][:, :, :, 10:19]
+        if which in (1, 2):
+            args[3] = args[1][:, :, :, 10:19]
+        if which == 3:
+            args[2], args[3] = args[1][:, :, :, 9:18], args[0][..., 11:20, :]
+        want = commit_reference(*(t.cpu() for t in args))
+        if layers == 1:
+            lens = commit_draft(*(t[0] for t in args[:4]), *args[4:])
+        else:
+            lens = commit_draft(*args)
+        for got, ref in zip((args[0], args[1], lens), want, strict=True):
+            assert torch.equal(got.cpu(), ref)
+    check_device_status()
+
+
+@pytest.mark.gpu
+@gpu
+def test_commit_copies_no_tree_beside_the_cache() -> None:
+    """Trees in the caches' memory but apart from them (rows behind them, keys and values side by side) are read in place."""
+    for layout in range(3):
+        args = [t.cuda() for t in commit_problem(2, 3, 2, 6, 20, 64, torch.float16, seed=10)]
+        want = commit_reference(*(t.cpu() for t in args))
+        if layout == 0:
+            for cache, tree in ((0, 2), (1, 3)):
+                both = torch.cat((args[cache], args[tree]), 3)
+                args[cache], args[tree] = both[:, :, :, :20], both[:, :, :, 20:]
+        elif layout == 1:
+            for cache, tree in ((0, 2), (1, 3)):
+                both = torch.cat((args[cache], args[tree]), 3).transpose(2, 3).contiguous().transpose(2, 3)
+                args[cache], args[tree] = both[:, :, :, :20], both[:, :, :, 20:]
+        else:
+            both = torch.stack((torch.cat((args[0], args[2]), 3), torch.cat((args[1], args[3]), 3)), 4)
+            args[0], args[1] = both[:, :, :, :20, 0], both[:, :, :, :20, 1]
+            args[2], args[3] = both[:, :, :, 20:, 0], both[:, :, :, 20:, 1]
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        lens = commit_draft(*args)
+        assert torch.cuda.memory_stats()["allocation.all.allocated"] == before + 1  # the new lengths
+        for got, ref in zip((args[0], args[1], lens), want, strict=True):
+            assert torch.equal(got.cpu(), ref)
     check_device_status()

@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 
@@ -343,6 +344,48 @@ PyObject* py_verify_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Whether index differences in [-(b_n - 1), a_n - 1] of each dimension (largest
+// stride first) add up to `d` elements.  Nested strides leave two or three
+// differences a dimension; `budget` ends the search of others, with a yes.
+struct Span {
+  int64_t stride, a_n, b_n;
+};
+bool meets(const Span* s, int dims, int64_t d, int* budget) {
+  if (dims == 0) return d == 0;
+  if (--*budget < 0) return true;
+  int64_t lo = 0, hi = 0;  // of what the further dimensions add
+  for (int i = 1; i < dims; ++i) lo -= (s[i].b_n - 1) * s[i].stride, hi += (s[i].a_n - 1) * s[i].stride;
+  if (s[0].stride == 0) return meets(s + 1, dims - 1, d, budget);
+  for (int64_t x = std::max(-(s[0].b_n - 1), (d - hi) / s[0].stride - 1); x < s[0].a_n && d - x * s[0].stride >= lo; ++x)
+    if (d - x * s[0].stride <= hi && meets(s + 1, dims - 1, d - x * s[0].stride, budget)) return true;
+  return false;
+}
+
+// Whether two tensors of as many dimensions and one type may have an element in
+// common.  Certain for tensors far apart and for views of one layout (rows of one
+// buffer, keys beside values); else yes.
+bool may_overlap(const Tensor& a, const Tensor& b) {
+  const char* pa = static_cast<const char*>(a.const_data_ptr());
+  const char* pb = static_cast<const char*>(b.const_data_ptr());
+  const int64_t bytes = a.element_size();
+  int64_t end_a = 1, end_b = 1;
+  Span spans[5];
+  int dims = 0;
+  bool alike = true;
+  for (int64_t i = 0; i < a.dim(); ++i) {
+    end_a += (a.size(i) - 1) * a.stride(i);
+    end_b += (b.size(i) - 1) * b.stride(i);
+    if (a.size(i) == 1 && b.size(i) == 1) continue;
+    alike = alike && (a.size(i) == 1 || b.size(i) == 1 || a.stride(i) == b.stride(i));
+    spans[dims++] = {a.size(i) > 1 ? a.stride(i) : b.stride(i), a.size(i), b.size(i)};
+  }
+  if (pa + end_a * bytes <= pb || pb + end_b * bytes <= pa) return false;
+  if (!alike || (pb - pa) % bytes != 0) return true;
+  std::sort(spans, spans + dims, [](const Span& x, const Span& y) { return x.stride > y.stride; });
+  int budget = 1000;
+  return meets(spans, dims, (pb - pa) / bytes, &budget);
+}
+
 PyObject* py_commit_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arity(n, 7)) return nullptr;
@@ -359,6 +402,11 @@ PyObject* py_commit_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
       kt.size(first) != batch || kt.size(first + 1) != heads || kt.size(first + 3) != dim || nodes == 0 ||
       nodes > kMaxNodes || dim % 8 != 0 || dim > 256)
     Py_RETURN_NONE;
+  // Drafts kept among the rows that are written: from a copy of them, for the
+  // kernel reads and writes rows in any order.
+  for (Tensor* t : {&kt, &vt})
+    if (like(*t, k.scalar_type(), k) && like(v, k.scalar_type(), k) && (may_overlap(k, *t) || may_overlap(v, *t)))
+      *t = t->clone(at::MemoryFormat::Contiguous);
   int64_t strides[16] = {};
   const Tensor* all[4] = {&k, &v, &kt, &vt};
   for (int i = 0; i < 4; ++i) {
@@ -384,6 +432,18 @@ PyObject* py_commit_draft(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// For the tests: of tensors on any device.
+PyObject* py_may_overlap(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 2)) return nullptr;
+  Tensor a, b;
+  TORCH_CHECK(tensor_arg(args[0], &a) && tensor_arg(args[1], &b) && a.dim() == b.dim() && a.dim() <= 5 && a.numel() > 0 &&
+                  b.numel() > 0 && a.scalar_type() == b.scalar_type(),
+              "may_overlap: two tensors of up to 5 dimensions and one type");
+  return PyBool_FromLong(may_overlap(a, b));
+  END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyMethodDef method(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
@@ -392,6 +452,7 @@ PyMethodDef method(const char* name) {
 PyMethodDef methods[] = {
     method<py_rotary>("rotary"),           method<py_tree_attention>("tree_attention"),
     method<py_verify_draft>("verify_draft"), method<py_commit_draft>("commit_draft"),
+    method<py_may_overlap>("may_overlap"),
     {nullptr, nullptr, 0, nullptr},
 };
 

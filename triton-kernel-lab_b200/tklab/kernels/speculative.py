@@ -173,7 +173,8 @@ def commit_draft(
     Row ``path[b, i]`` (``i < path_lens[b]``) of ``k_tree`` and ``v_tree`` goes to
     cache row ``kv_lens[b] + i``.  Caches (batch, kv_heads, seq_kv, head_dim) with
     trees (batch, kv_heads, nodes, head_dim), or both with a leading layers
-    dimension: all layers are then written in one launch.  Rows are copied as
+    dimension: all layers are then written in one launch.  Trees that overlap
+    the caches (drafts kept among their rows) are copied first.  Rows are copied as
     data, no gradient goes through the cache.  Rows that the cache has no room
     for are left out and the returned length stops at ``seq_kv``; ``path_lens``
     outside 0..nodes and ``kv_lens`` outside 0..seq_kv are clamped; in either case
