@@ -7,10 +7,11 @@ it travels with the source tree.  A second, test-only library,
 tcgen05 operand forms and of the FMA-pipe exponential), is built beside it;
 only the tests load it.  ``tklab/_lib/_tklab_tensors.so``
 (``csrc/binding/``) is a Python extension that calls the library's serving
-entries on torch tensors; it is compiled against the installed torch.  Run
-``python build_native.py`` or call :func:`build`.  Each library is rebuilt
-only when one of its sources or headers is newer than it, unless ``force`` is
-set.
+entries on torch tensors; it is compiled against the installed torch, which a
+stamp in it names.  Run ``python build_native.py`` or call :func:`build`.
+Each library is rebuilt only when one of its sources or headers is newer than
+it (the extension also when its stamp is not this environment's), unless
+``force`` is set.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ import argparse
 import os
 import shutil
 import subprocess
+import sys
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -117,9 +119,14 @@ def _build_binding(force: bool, verbose: bool) -> None:
 
     import torch
 
+    if str(ROOT) not in sys.path:
+        sys.path.insert(0, str(ROOT))
+    from tklab._tensors import STAMP_MARK, binding_stamp, stamp_of
+
     deps = [BINDING_SOURCE, INCLUDE / "tklab_attn.h"]
     if not force and BINDING_PATH.exists() and all(d.stat().st_mtime <= BINDING_PATH.stat().st_mtime for d in deps):
-        return
+        if stamp_of(BINDING_PATH) == binding_stamp():
+            return
     gxx = shutil.which("g++")
     if gxx is None:
         raise RuntimeError("g++ not found: put it on PATH")
@@ -133,6 +140,7 @@ def _build_binding(force: bool, verbose: bool) -> None:
     cmd = [
         gxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        f'-DTKLAB_STAMP="{STAMP_MARK}{binding_stamp()}"',
         *[arg for path in includes for arg in ("-isystem", str(path))],
         str(BINDING_SOURCE), "-o", str(tmp),
         "-L", str(LIB_DIR), "-l:" + LIB_PATH.name, "-Wl,-rpath,$ORIGIN",

@@ -458,6 +458,10 @@ PyMethodDef methods[] = {
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tklab_tensors", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
+// What this file was compiled for (build_native.py), which is looked up before
+// the extension is loaded.
+[[gnu::used]] const char stamp[] = TKLAB_STAMP;
+
 }  // namespace
 
 PyMODINIT_FUNC PyInit__tklab_tensors() { return PyModule_Create(&module); }

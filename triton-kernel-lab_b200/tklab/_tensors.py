@@ -12,14 +12,30 @@ from __future__ import annotations
 
 import importlib.util
 import sys
+import sysconfig
 from pathlib import Path
 from types import ModuleType
 
-import torch  # noqa: F401  (the extension links to the libraries that this loads)
+import torch  # (the extension links to the libraries that this loads)
 
 from tklab import _native
 
 BINDING_PATH = Path(__file__).resolve().parent / "_lib" / "_tklab_tensors.so"
+
+
+STAMP_MARK = "built for: "
+
+
+def binding_stamp() -> str:
+    """What an extension has to have been compiled for to be loaded here: torch, its C++ ABI, CUDA, Python."""
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    return f"torch {torch.__version__}, cxx11 abi {abi}, cuda {torch.version.cuda}, {sysconfig.get_config_var('SOABI')}"
+
+
+def stamp_of(path: Path) -> str:
+    """The stamp that the build put into the extension at ``path``, without loading it."""
+    _, mark, rest = path.read_bytes().partition(STAMP_MARK.encode())
+    return rest.partition(b"\0")[0].decode(errors="replace") if mark else "an unknown environment"
 
 
 def load() -> ModuleType:
@@ -30,6 +46,11 @@ def load() -> ModuleType:
             raise RuntimeError(
                 f"{BINDING_PATH.name} is not built: run `python triton-kernel-lab_b200/build_native.py` "
                 "(or __graft_entry__.build()) before using the serving operators"
+            )
+        if stamp_of(BINDING_PATH) != binding_stamp():
+            raise RuntimeError(
+                f"{BINDING_PATH.name} was built for {stamp_of(BINDING_PATH)}, this is {binding_stamp()}: run "
+                "`python triton-kernel-lab_b200/build_native.py`"
             )
         _native.load()
         spec = importlib.util.spec_from_file_location(name, BINDING_PATH)
