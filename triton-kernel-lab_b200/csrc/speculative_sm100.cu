@@ -145,8 +145,9 @@ __device__ __forceinline__ int word_shift(const void* p, int64_t at) {
 // Measured, per call: 18.3 us for 128 chains of 5 over 50257 float32 entries
 // (4.2 TB/s; 16.0 us, 4.8 TB/s for 50304, whose rows start on 16 bytes);
 // 10.4 us for 32 trees of 64 over 128000 bf16 entries, 3 us of it the tree (1.7
-// the loads of parents and tokens and then of their probabilities); 4.6 us for one chain of 6 over 32000.  With 128 or 256 threads a CTA
-// and more CTAs the first took 18.1 to 19.0 us, the second 11.4 to 15.9.
+// the loads of parents and tokens and then of their probabilities); 4.6 us for
+// one chain of 6 over 32000.  With 128 or 256 threads a CTA and more CTAs the
+// first took 18.1 to 19.0 us, the second 11.4 to 15.9.
 //
 // The race is run on w times the hardware reciprocal of e (a few operations an
 // element, no branch); a thread then divides for its own best only, or, if its

@@ -38,17 +38,18 @@
 // Few items with few tiles are bound by latency, not by bytes: there each item
 // gets a CTA to itself (one launch, no scan, no workspace; TreePlan::whole,
 // tree_grid).  Rows are not copied then: joining the copies takes longer than
-// they save on a few tiles.  (Clusters of CTAs that share an item and join it over distributed
-// shared memory were no quicker than the second launch: 12.0 against 12.3 us a
-// call for 8 items of 9 tiles, 24.7 against 22.1 at 256 rows.)
+// they save on a few tiles.  (Clusters of CTAs that share an item and join it
+// over distributed shared memory were no quicker than the second launch: 12.0
+// against 12.3 us a call for 8 items of 9 tiles, 24.7 against 22.1 at 256 rows.)
 //
 // Cache rows past kv_lens, tree rows past tree_sizes and, for a row, nodes that
 // it does not attend may hold anything: the scores of masked keys are replaced
 // before they are used, and in shared memory a V tile's rows past the last valid
 // key are cleared, and in tree tiles what is not finite (0 times it would be NaN
 // in the product); the rows that attend the latter get it added at the end.
-// (With copies an infinite value of a cache row, which every row attends, makes
-// NaN instead of infinity.)
+// An infinite value in a cache row, which every row attends, makes its column
+// infinite, or NaN where a weight is 0: one that underflowed, or a copy's for
+// the keys of the others.
 //
 // Measured, per call (cache bytes; useful flops), 32 sequences of 4096 to 8192
 // keys, 8 KV heads of 128, bf16:
@@ -631,7 +632,7 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
   uint64_t* drained = pv_done + 1;          // after a wait that gave up: every product
   CtaControl* ctl = reinterpret_cast<CtaControl*>(smem + C::kCtlOff);
   // Values that are not finite were taken out of a tree tile of this CTA.  Warp 3
-  // sets it before v_ok of the tile, which the softmax warps wait for.
+  // sets it before v_ok of the tile; it is read after o_final of its segment.
   volatile int* patched = reinterpret_cast<int*>(smem + C::kCtlOff + sizeof(CtaControl));
   int* first = reinterpret_cast<int*>(smem + C::kCtlOff + 16);  // this CTA's run: b, h, u, length; the runs' length
   int* loads = first + 5;  // [3]: tiles of K (warp 0) and V (warp 2) and segments' Q (warp 3) that were asked for
@@ -675,7 +676,7 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
     for (int i = lane; i < C::kNumBars; i += 32) {
       uint64_t* bar = q_full + i;
       const bool by_warps = (bar >= p_ready && bar < p_ready + 2) || (bar >= o_empty && bar < o_empty + 4);
-      mbar_init(bar, by_warps ? 4 : 1);
+      mbar_init(bar, by_warps ? 4 : bar >= o_final && bar < o_final + 2 ? 2 : 1);
     }
     if (lane == 0) {
       ctl->abort = 0;
@@ -928,7 +929,12 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
             issue_pv(buf, ob, st, j > 0);
             if (x == kT - 1) commit(&v_empty[st]);
             if constexpr (kLook == 2) commit(pv_done);
-            if (j == n - 1) commit(&o_final[C::kEpi ? ob : x]);
+            if (j == n - 1) {
+              // The products' arrival, and one of this warp, which has waited for the
+              // segment's v_ok: after both, `patched` is what warp 3 made it.
+              commit(&o_final[C::kEpi ? ob : x]);
+              if (lane == 0) mbar_arrive(&o_final[C::kEpi ? ob : x]);
+            }
             if (j + kLook < n) {
               if constexpr (kT == 1) {
                 if (!(ok = scores(j + kLook))) break;
@@ -1013,9 +1019,6 @@ __global__ void __launch_bounds__(TreeCfg<D, kT, kRep>::kThreads, 1)
           }
           tmem_wait_st();
         }
-        // (P V needs the tile's V anyhow; before p_ready, so that v_ok cannot be a
-        // phase further.)
-        if (on_tree && !(ok = warp_wait(&v_ok[g % C::kVStages], (g / C::kVStages) & 1, ctl, timeout_ns, status, 16))) break;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[buf]);

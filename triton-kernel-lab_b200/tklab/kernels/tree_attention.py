@@ -20,7 +20,6 @@ from tklab._tensors import binding, contiguous, dense, distinct, require_cache
 from tklab.kernels.flash_attention import _NATIVE_DTYPE, _after_launch
 
 MAX_TREE_NODES = 256
-TREE_HEAD_DIMS = tuple(range(8, 129, 8))
 
 
 def check_parents(parents: torch.Tensor | None, batch: int, nodes: int, device: torch.device) -> None:
