@@ -54,16 +54,23 @@
 // Measured, per call (cache bytes; useful flops), 32 sequences of 4096 to 8192
 // keys, 8 KV heads of 128, bf16:
 //   32 rows    134 us   6.0 TB/s, 94 % of a copy
-//   256 rows   212 us   4.0 TB/s, 980 TFLOP/s: two tiles' softmax and their
-//              products in turn, the tensor pipe 48 % active, the device at its
-//              power limit (1.45 GHz; 262 us when kept there)
+//   256 rows   218 us   3.9 TB/s, 950 TFLOP/s on a rested device: two tiles'
+//              softmax and their products in turn, the tensor pipe 45 %
+//              active; called without a pause, at the power limit (1.45 GHz),
+//              255 to 267 us
 // and 2 sequences of 100000 to 131000 keys, 4 KV heads of 128, 104 rows, fp16:
-//   84 us      5.6 TB/s, 88 % of a copy.
-// The smallest call (8 items of 1000 keys, 32 rows) takes 9.2 us: two launches
+//   83 us      5.7 TB/s, 89 % of a copy; 93 to 102 us at the power limit.
+// The smallest call (8 items of 1000 keys, 32 rows) takes 9.1 us: two launches
 // and a chain of loads, products and a join.  For 256 rows none of these was
-// quicker than 218 to 223 us at the time: P announced in two parts, so that P V starts under the second
-// part's exponentials (221 us); S and P in halves (232); S read twice, in loops
-// that need fewer registers (227); two softmax warpgroups a tile (315).
+// quicker than 218 to 223 us at the time: P announced in two parts, so that P V
+// starts under the second part's exponentials (221 us); S and P in halves (232);
+// S read twice, in loops that need fewer registers (227); two softmax
+// warpgroups a tile (315).
+//
+// What numbers that are not finite cost, in such times: the search of the tree
+// tiles' V, the maximum that carries NaN and the additions at the end 1.5 us of
+// 62 for 8 sequences of 256 rows (2.5 %), 0.2 of 9 for the smallest call, nothing
+// that can be told for the long cache.
 #include <algorithm>
 
 #include "attn_launch.h"
