@@ -193,7 +193,8 @@ bool tensor_arg(PyObject* o, Tensor* t, bool optional = false) {
 // The operators know no forward mode: a tangent that would be lost is an error.
 void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
   for (const Tensor* t : tensors)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || t->unsafeGetTensorImpl()->autograd_meta() == nullptr || !t->_fw_grad(0).defined(),
+                                what, " has no forward-mode derivative");
 }
 
 PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
@@ -246,13 +247,9 @@ struct NoDerivative : torch::autograd::Node {
   }
 };
 
-void mark_no_derivative(std::initializer_list<Tensor> inputs, std::initializer_list<Tensor> outputs) {
-  if (!at::GradMode::is_enabled()) return;
-  bool needed = false;
-  for (const Tensor& t : inputs) needed = needed || t.requires_grad();
-  if (!needed) return;
+void mark_no_derivative(const torch::autograd::variable_list& inputs, const torch::autograd::variable_list& outputs) {
   std::shared_ptr<torch::autograd::Node> node(new NoDerivative(), torch::autograd::deleteNode);
-  node->set_next_edges(torch::autograd::collect_next_edges(torch::autograd::variable_list(inputs)));
+  node->set_next_edges(torch::autograd::collect_next_edges(inputs));
   for (const Tensor& t : outputs)
     if (t.defined()) torch::autograd::set_history(t, node);
 }
@@ -299,7 +296,9 @@ PyObject* py_tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
                      bytes > 0 ? workspace.data_ptr() : nullptr, bytes, batch, q_heads, kv_heads, nodes, rows, dim,
                      attn_dtype(q), static_cast<float>(scale), on.handle()),
         "tk_tree_attn");
-  mark_no_derivative({q, k, v, kt, vt}, {out, lse});
+  if (at::GradMode::is_enabled() &&
+      (q.requires_grad() || k.requires_grad() || v.requires_grad() || kt.requires_grad() || vt.requires_grad()))
+    mark_no_derivative({q, k, v, kt, vt}, {out, lse});
   return return_lse ? tuple_of({out, lse}) : THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
@@ -368,18 +367,21 @@ bool may_overlap(const Tensor& a, const Tensor& b) {
   const char* pa = static_cast<const char*>(a.const_data_ptr());
   const char* pb = static_cast<const char*>(b.const_data_ptr());
   const int64_t bytes = a.element_size();
-  int64_t end_a = 1, end_b = 1;
+  const auto end = [](const Tensor& t) {
+    const auto sizes = t.sizes(), strides = t.strides();
+    int64_t n = 1;
+    for (size_t i = 0; i < sizes.size(); ++i) n += (sizes[i] - 1) * strides[i];
+    return n;
+  };
+  if (pa < pb ? pa + end(a) * bytes <= pb : pb + end(b) * bytes <= pa) return false;
   Span spans[5];
   int dims = 0;
   bool alike = true;
   for (int64_t i = 0; i < a.dim(); ++i) {
-    end_a += (a.size(i) - 1) * a.stride(i);
-    end_b += (b.size(i) - 1) * b.stride(i);
     if (a.size(i) == 1 && b.size(i) == 1) continue;
     alike = alike && (a.size(i) == 1 || b.size(i) == 1 || a.stride(i) == b.stride(i));
     spans[dims++] = {a.size(i) > 1 ? a.stride(i) : b.stride(i), a.size(i), b.size(i)};
   }
-  if (pa + end_a * bytes <= pb || pb + end_b * bytes <= pa) return false;
   if (!alike || (pb - pa) % bytes != 0) return true;
   std::sort(spans, spans + dims, [](const Span& x, const Span& y) { return x.stride > y.stride; });
   int budget = 1000;

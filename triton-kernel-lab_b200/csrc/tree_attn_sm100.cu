@@ -597,6 +597,7 @@ __device__ __forceinline__ void finish_copies(bool ok, uint32_t o_addr, int r, b
     else if (lse != nullptr)
       lse[item_row + jrow] = jl == 0.0f ? -INFINITY : jtop + lg2(jl);
   }
+  __syncwarp();
   named_barrier_sync(1, 128);  // before the next segment's ml and columns
 }
 
